@@ -133,10 +133,11 @@ def _rows(n, heads, dim, dtype, gen):
 
 def _codes(x, kind):
     """(codes as float64, fp32 scales) of rows x."""
-    amax = x.float().abs().amax(-1)
-    fine = amax >= TINY
-    scale = torch.where(fine, amax / QMAX[kind], torch.zeros_like(amax))
-    inverse = torch.where(fine, QMAX[kind] / torch.where(fine, amax, torch.ones_like(amax)), torch.zeros_like(amax))
+    amax = x.double().abs().amax(-1)
+    fine, most = amax >= TINY, torch.full_like(amax, QMAX[kind])
+    # both quotients are rounded once to 32 bits: they are part of the format
+    scale = torch.where(fine, amax / most, 0.0).float()
+    inverse = torch.where(fine, most / torch.where(fine, amax, 1.0), 0.0).float()
     y = x.double() * inverse.double().unsqueeze(-1)
     if kind != "fp8":
         return torch.round(y), scale
