@@ -9,7 +9,8 @@ __version__ = "0.1.0"
 
 
 def __getattr__(name):
-    if name in ("decoding_attn_fwd", "dmha_fwd", "dmla_fwd", "paged_fwd", "merge_partials"):
+    if name in ("decoding_attn_fwd", "dmha_fwd", "dmla_fwd", "paged_fwd", "merge_partials", "kv_cache_write",
+                "kv_cache_read", "quantized_fwd"):
         from . import interface
         return getattr(interface, name)
     raise AttributeError(name)

@@ -13,7 +13,8 @@ LIB_PATH = os.environ.get("DA_LIB_PATH") or os.path.join(_PKG, "libdecoding_attn
 DA_OK, DA_ERR_INVALID_ARG, DA_ERR_UNSUPPORTED, DA_ERR_WORKSPACE, DA_ERR_CUDA, DA_ERR_TIMEOUT = range(6)
 
 EXPORTS = ["da_decode_fwd", "da_decode_fwd_host", "da_decode_fwd_static", "da_static_scratch_bytes", "da_decode_workspace_bytes", "da_decode_num_splits", "da_plan_num_splits",
-           "da_merge_partials", "da_exchange_merge", "da_exchange_merge_bounded", "da_exchange_buffer_bytes", "da_set_profile_events", "da_selftest_wait_timeout", "da_device_status", "da_status_string", "da_last_error", "da_launch_count"]
+           "da_merge_partials", "da_exchange_merge", "da_exchange_merge_bounded", "da_exchange_buffer_bytes", "da_kv_cache_write", "da_kv_cache_read", "da_quant_decode_fwd",
+           "da_quant_decode_workspace_bytes", "da_set_profile_events", "da_selftest_wait_timeout", "da_device_status", "da_status_string", "da_last_error", "da_launch_count"]
 
 
 class DecodeArgs(ctypes.Structure):
@@ -35,6 +36,33 @@ class DecodeArgs(ctypes.Structure):
         ("block_table", ctypes.c_void_p), ("block_table_stride", ctypes.c_int64),
         ("page_size", ctypes.c_int32),
         ("kv_dtype", ctypes.c_int32), ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float),
+    ]
+
+
+class KvRowsArgs(ctypes.Structure):
+    """Mirror of ``da_kv_rows_args_t``."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("kv_dtype", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64), ("cache_rows", ctypes.c_int64), ("head_k", ctypes.c_int64), ("dim", ctypes.c_int64),
+        ("k_row_stride", ctypes.c_int64), ("v_row_stride", ctypes.c_int64), ("stream", ctypes.c_void_p),
+    ]
+
+
+class QuantDecodeArgs(ctypes.Structure):
+    """Mirror of ``da_quant_decode_args_t``."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("is_bf16", ctypes.c_int32), ("is_alibi", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p), ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("cu_seq_k", ctypes.c_void_p),
+        ("rows", ctypes.c_int64), ("batch", ctypes.c_int64), ("head_q", ctypes.c_int64), ("head_k", ctypes.c_int64),
+        ("dim", ctypes.c_int64), ("q_row_stride", ctypes.c_int64), ("o_row_stride", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p), ("block_table_stride", ctypes.c_int64), ("table_blocks", ctypes.c_int64),
+        ("page_size", ctypes.c_int32), ("softmax_scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
     ]
 
 
@@ -80,6 +108,13 @@ def lib():
         l.da_exchange_merge_bounded.argtypes = l.da_exchange_merge.argtypes + [ctypes.c_int64]
         l.da_exchange_buffer_bytes.restype = ctypes.c_size_t
         l.da_exchange_buffer_bytes.argtypes = [ctypes.c_int32, ctypes.c_int64, ctypes.c_int32]
+        for name in ("da_kv_cache_write", "da_kv_cache_read"):
+            getattr(l, name).restype = ctypes.c_int
+            getattr(l, name).argtypes = [ctypes.POINTER(KvRowsArgs)]
+        l.da_quant_decode_fwd.restype = ctypes.c_int
+        l.da_quant_decode_fwd.argtypes = [ctypes.POINTER(QuantDecodeArgs)]
+        l.da_quant_decode_workspace_bytes.restype = ctypes.c_size_t
+        l.da_quant_decode_workspace_bytes.argtypes = [ctypes.POINTER(QuantDecodeArgs)]
         l.da_set_profile_events.restype = None
         l.da_set_profile_events.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         l.da_selftest_wait_timeout.restype = ctypes.c_int

@@ -1,0 +1,260 @@
+// Rows of a quantised KV cache: writing them from 16-bit rows and reading them back.
+//
+// A row x is one token and one KV head, D values.  With Q the largest code of the format (448 for FP8 e4m3, 127
+// for int8, 7 for int4) and a = max |x|:
+//     scale = fl32(a / Q),   code = rn(x * fl32(Q / a)),   x is read back as rn(code * scale).
+// The product is rounded ONCE, from its exact value: for integers by an fma that adds 1.5 * 2^23 (whose ulp is 1),
+// for e4m3 by truncating to 24 bits with a sticky last bit before the hardware conversion -- so the codes are a
+// function of the definition and not of an order of operations.  Rows with a < 2^-100 become zeros with scale 0
+// (both quotients stay normal numbers); a row that holds an infinity or a NaN gets scale NaN and codes 0, so that
+// whatever reads it sees NaN.
+//
+// Bound: HBM.  A row costs 2D bytes on the 16-bit side and D (or D / 2) + 4 on the other; nothing is read twice.
+// A row belongs to L lanes of one warp that hold 8 values a piece (16-byte accesses on the 16-bit side), the maximum
+// is joined by xor shuffles inside these lanes, and a thread has kRows rows in flight, since the slot, the row
+// and (reading) the scale are a chain of two loads.
+#include "da_internal.h"
+#include "da_kv_rows.h"
+
+namespace da {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Lanes of a row and 8-value chunks of a lane.
+template <int D>
+struct RowCfg {
+    static constexpr int kLanes = D == 96 ? 4 : D / 8;
+    static constexpr int kChunks = D / 8 / kLanes;
+};
+
+template <int KVQ>
+__device__ __forceinline__ constexpr float code_max() {
+    return KVQ == 1 ? 448.0f : (KVQ == 2 ? 127.0f : 7.0f);
+}
+
+// x * inv rounded once to an integer; the low bits of the result are the code in two's complement.
+__device__ __forceinline__ uint32_t round_code(float x, float inv) {
+    return __float_as_uint(__fmaf_rn(x, inv, 12582912.0f));
+}
+// x * inv cut to 24 bits, with the last bit set when something was cut off: a second rounding to fewer bits then
+// gives what one rounding of the exact product would.
+__device__ __forceinline__ float product_sticky(float x, float inv) {
+    const float p = __fmul_rz(x, inv);
+    const float rest = __fmaf_rn(x, inv, -p);
+    return __uint_as_float(__float_as_uint(p) | (rest != 0.0f ? 1u : 0u));
+}
+
+template <int KVQ>
+__device__ __forceinline__ void store_codes(uint8_t *dst, const float (&x)[8], float inv) {
+    if (KVQ == 1) {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 a = {product_sticky(x[4 * i], inv), product_sticky(x[4 * i + 1], inv)};
+            const float2 b = {product_sticky(x[4 * i + 2], inv), product_sticky(x[4 * i + 3], inv)};
+            w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+                   ((uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16);
+        }
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+    } else if (KVQ == 2) {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t lo = __byte_perm(round_code(x[4 * i], inv), round_code(x[4 * i + 1], inv), 0x0040);
+            const uint32_t hi = __byte_perm(round_code(x[4 * i + 2], inv), round_code(x[4 * i + 3], inv), 0x0040);
+            w[i] = __byte_perm(lo, hi, 0x5410);
+        }
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+    } else {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w |= (round_code(x[i], inv) & 15u) << (4 * i);
+        *reinterpret_cast<uint32_t *>(dst) = w;
+    }
+}
+
+// blockIdx.y: 0 the K rows, 1 the V rows.  Row r = token * head_k + head.
+template <typename T, int D, int KVQ, int kRows>
+__global__ void __launch_bounds__(kThreads) da_kv_write_kernel(const KvRowsParams p) {
+    using C = RowCfg<D>;
+    constexpr int kRowBytes = KVQ == 3 ? D / 2 : D;
+    constexpr int kBlockRows = kThreads / C::kLanes;
+    const T *__restrict__ src = static_cast<const T *>(blockIdx.y ? p.v : p.k);
+    const long long src_stride = blockIdx.y ? p.v_row_stride : p.k_row_stride;
+    uint8_t *__restrict__ cache = static_cast<uint8_t *>(blockIdx.y ? p.v_cache : p.k_cache);
+    float *__restrict__ scales = blockIdx.y ? p.v_scale : p.k_scale;
+    const int lane = threadIdx.x % C::kLanes;
+    const uint32_t total = p.rows;
+    const uint32_t first = blockIdx.x * (uint32_t)(kBlockRows * kRows) + threadIdx.x / C::kLanes;
+    const unsigned group = C::kLanes == 32 ? 0xffffffffu
+                                           : ((1u << (C::kLanes & 31)) - 1u) << ((threadIdx.x & 31) / C::kLanes * C::kLanes);
+
+    uint4 raw[kRows][C::kChunks];
+    long long slot[kRows];
+    uint32_t head[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const uint32_t r = first + i * kBlockRows;
+        slot[i] = -1;
+        head[i] = 0;
+        if (r < total) {
+            const uint32_t token = r / (uint32_t)p.head_k;
+            head[i] = r - token * (uint32_t)p.head_k;
+            slot[i] = p.slots ? p.slots[token] : (long long)token;
+            const T *row = src + (long long)token * src_stride + (long long)head[i] * D;
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c) raw[i][c] = __ldcs(reinterpret_cast<const uint4 *>(row) + lane + c * C::kLanes);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        if (slot[i] < 0 || slot[i] >= p.cache_rows) continue;  // uniform over the lanes of a row
+        float x[C::kChunks][8];
+        uint32_t top = 0;  // the magnitudes compare as integers; infinities and NaN come out above every number
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c) {
+            unpack8<T>(raw[i][c], x[c]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[c][e]) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int d = 1; d < C::kLanes; d <<= 1) top = max(top, __shfl_xor_sync(group, top, d));
+        const float amax = __uint_as_float(top);
+        float scale = 0.0f, inv = 0.0f;
+        if (top >= 0x7f800000u) {
+            scale = __uint_as_float(0x7fffffffu);
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[c][e] = 0.0f;
+        } else if (top >= 0x0d800000u) {  // 2^-100
+            scale = __fdiv_rn(amax, code_max<KVQ>());
+            inv = __fdiv_rn(code_max<KVQ>(), amax);
+        }
+        const long long row = slot[i] * p.head_k + head[i];
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c)
+            store_codes<KVQ>(cache + row * kRowBytes + (lane + c * C::kLanes) * (KVQ == 3 ? 4 : 8), x[c], inv);
+        if (lane == 0) scales[row] = scale;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T *dst, const float (&x)[8]) {
+    uint4 w;
+    T *h = reinterpret_cast<T *>(&w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = from_float<T>(x[e]);
+    __stcs(reinterpret_cast<uint4 *>(dst), w);
+}
+template <>
+__device__ __forceinline__ void store8<float>(float *dst, const float (&x)[8]) {
+    __stcs(reinterpret_cast<float4 *>(dst), make_float4(x[0], x[1], x[2], x[3]));
+    __stcs(reinterpret_cast<float4 *>(dst) + 1, make_float4(x[4], x[5], x[6], x[7]));
+}
+
+template <typename T, int D, int KVQ, int kRows>
+__global__ void __launch_bounds__(kThreads) da_kv_read_kernel(const KvRowsParams p) {
+    using C = RowCfg<D>;
+    constexpr int kRowBytes = KVQ == 3 ? D / 2 : D;
+    constexpr int kBlockRows = kThreads / C::kLanes;
+    T *__restrict__ dst = static_cast<T *>(blockIdx.y ? p.v : p.k);
+    const long long dst_stride = blockIdx.y ? p.v_row_stride : p.k_row_stride;
+    const uint8_t *__restrict__ cache = static_cast<const uint8_t *>(blockIdx.y ? p.v_cache : p.k_cache);
+    const float *__restrict__ scales = blockIdx.y ? p.v_scale : p.k_scale;
+    const int lane = threadIdx.x % C::kLanes;
+    const uint32_t total = p.rows;
+    const uint32_t first = blockIdx.x * (uint32_t)(kBlockRows * kRows) + threadIdx.x / C::kLanes;
+
+    uint2 raw[kRows][C::kChunks];
+    float scale[kRows];
+    long long slot[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const uint32_t r = first + i * kBlockRows;
+        slot[i] = r < total ? (p.slots ? p.slots[r / (uint32_t)p.head_k] : (long long)(r / (uint32_t)p.head_k)) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        scale[i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c) raw[i][c] = make_uint2(0, 0);
+        if (slot[i] < 0 || slot[i] >= p.cache_rows) continue;
+        const uint32_t r = first + i * kBlockRows;
+        const long long row = slot[i] * p.head_k + r % (uint32_t)p.head_k;
+        scale[i] = scales[row];
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c) {
+            const uint8_t *q = cache + row * kRowBytes + (lane + c * C::kLanes) * (KVQ == 3 ? 4 : 8);
+            if (KVQ == 3) raw[i][c].x = __ldcs(reinterpret_cast<const uint32_t *>(q));
+            else raw[i][c] = __ldcs(reinterpret_cast<const uint2 *>(q));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const uint32_t r = first + i * kBlockRows;
+        if (r >= total) continue;
+        const uint32_t token = r / (uint32_t)p.head_k, head = r - token * (uint32_t)p.head_k;
+        T *row = dst + (long long)token * dst_stride + (long long)head * D;
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c) {
+            float x[8];
+            load_chunk8<__half, KVQ>(reinterpret_cast<const uint8_t *>(&raw[i][c]), x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], scale[i]);
+            store8<T>(row + (lane + c * C::kLanes) * 8, x);
+        }
+    }
+}
+
+// Rows of a thread.  Few rows: one each, to spread them over the SMs.
+template <typename T, int D, int KVQ>
+cudaError_t launch_rows(const KvRowsParams &p, bool write, cudaStream_t s) {
+    constexpr uint32_t kBlockRows = kThreads / RowCfg<D>::kLanes;
+    const bool many = p.rows > 4u * kBlockRows * 148u;
+    const uint32_t per_block = kBlockRows * (many ? 4u : 1u);
+    const dim3 grid((p.rows + per_block - 1) / per_block, 2);
+    if (write) {
+        if constexpr (!std::is_same<T, float>::value) {
+            if (many) da_kv_write_kernel<T, D, KVQ, 4><<<grid, kThreads, 0, s>>>(p);
+            else da_kv_write_kernel<T, D, KVQ, 1><<<grid, kThreads, 0, s>>>(p);
+        } else {
+            return cudaErrorInvalidValue;
+        }
+    } else if (many) {
+        da_kv_read_kernel<T, D, KVQ, 4><<<grid, kThreads, 0, s>>>(p);
+    } else {
+        da_kv_read_kernel<T, D, KVQ, 1><<<grid, kThreads, 0, s>>>(p);
+    }
+    count_launch();
+    return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch_kind(const KvRowsParams &p, int kvq, bool write, cudaStream_t s) {
+    if (kvq == 1) return launch_rows<T, D, 1>(p, write, s);
+    if (kvq == 2) return launch_rows<T, D, 2>(p, write, s);
+    return launch_rows<T, D, 3>(p, write, s);
+}
+
+template <typename T>
+cudaError_t launch_dim(const KvRowsParams &p, int dim, int kvq, bool write, cudaStream_t s) {
+    switch (dim) {
+        case 64: return launch_kind<T, 64>(p, kvq, write, s);
+        case 96: return launch_kind<T, 96>(p, kvq, write, s);
+        case 128: return launch_kind<T, 128>(p, kvq, write, s);
+        case 256: return launch_kind<T, 256>(p, kvq, write, s);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_kv_rows(const KvRowsParams &p, int dim, int x_dtype, int kvq, bool write, cudaStream_t s) {
+    if (x_dtype == 0) return launch_dim<__half>(p, dim, kvq, write, s);
+    if (x_dtype == 1) return launch_dim<__nv_bfloat16>(p, dim, kvq, write, s);
+    return launch_dim<float>(p, dim, kvq, write, s);
+}
+
+}  // namespace da

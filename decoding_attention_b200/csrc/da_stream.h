@@ -1,0 +1,87 @@
+// Launch parameters of the key-stream decode kernels (da_stream_kernel.cuh) and of the merge behind them.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace da {
+
+// The keys of all sequences, laid end to end as cu_seq_k has them, are cut into `spans` equal spans, one per CTA
+// (and head block).  The cut between two spans falls on a multiple of kSpanKeys keys of its sequence.
+constexpr int kSpanKeys = 32;
+
+struct StreamParams {
+    const void *q;                 // [batch, head_q, dim]
+    const void *k, *v;             // [rows, head_k, dim] elements or codes
+    const float *k_scale, *v_scale;  // [rows, head_k], quantised caches only
+    const int *cu_seq_k;           // [batch + 1]
+    const int *block_table;        // optional [batch, table_stride]
+    void *o;                       // [batch, head_q, dim]; NULL: whole sequences go to own_o / own_lse
+    float *lse;                    // optional [batch, head_q]
+    float *own_o, *own_lse;        // fp32 results of sequences that one CTA holds, when o is NULL
+    float *part_o, *part_lse;      // pieces of the others [spans][2][head_q][dim], [spans][2][head_q]
+    long long q_row_stride, k_row_stride, v_row_stride, o_row_stride;  // in elements
+    long long rows;                // rows of k and v (pages * page_size); rows outside are masked
+    long long table_stride;
+    int table_blocks;              // pages of a table row
+    int page_shift;
+    int batch, head_q, head_k, group;
+    int chunks;                    // warps that share a KV head (each has up to 8 NT of its query heads)
+    int head_warps, key_warps;     // a CTA's eight warps: so many (KV head, chunk) streams x so many parts of the keys
+    int spans, min_span;           // CTAs along the keys; no span is shorter than min_span keys
+    int is_alibi, q_bf16;
+    float scale_log2;              // softmax scale * log2(e)
+};
+
+// kind: 0 the type of q, 1 FP8 e4m3, 2 int8, 3 int4.
+struct StreamShape {
+    int heads;         // query heads of a warp (8 NT)
+    int ctas_per_sm;
+};
+StreamShape stream_shape_d64(int kind, int group);
+StreamShape stream_shape_d96(int kind, int group);
+StreamShape stream_shape_d128(int kind, int group);
+StreamShape stream_shape_d256(int kind, int group);
+cudaError_t launch_stream_d64(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
+cudaError_t launch_stream_d96(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
+cudaError_t launch_stream_d128(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
+cudaError_t launch_stream_d256(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
+
+// o = softmax-weighted sum of a row's pieces: those of the key stream, and (shared prefix) `prefix_parts` more.
+struct StreamMergeParams {
+    StreamParams s;
+    const float *prefix_o, *prefix_lse;  // [prefix_parts][batch][head_q][dim], [prefix_parts][batch][head_q]
+    int prefix_parts;
+    int dim;
+    void *o;      // [batch, head_q, dim], rows s.o_row_stride apart
+    float *lse;   // optional [batch, head_q]
+};
+cudaError_t launch_stream_merge(const StreamMergeParams &p, cudaStream_t s, bool overlap);
+
+// The cut of the batch's keys into spans, the same in the stream kernel and in the merge.
+struct SpanPlan {
+    long long first, total;  // cu_seq_k[0], keys of the batch
+    long long keys;          // of a span
+};
+#ifdef __CUDACC__
+__device__ __forceinline__ SpanPlan span_plan(const StreamParams &p) {
+    SpanPlan s;
+    s.first = p.cu_seq_k[0];
+    s.total = p.cu_seq_k[p.batch] - s.first;
+    if (s.total < 0) s.total = 0;
+    long long keys = (s.total + p.spans - 1) / p.spans;
+    if (keys < p.min_span) keys = p.min_span;
+    s.keys = (keys + kSpanKeys - 1) / kSpanKeys * kSpanKeys;
+    return s;
+}
+// Keys [begin, end) that span i has of a sequence of `len` keys that starts at `start` on the common axis; the cuts are
+// moved down to a multiple of kSpanKeys keys of the sequence.
+__device__ __forceinline__ void span_piece(const SpanPlan &s, long long i, long long start, int len, int &begin, int &end) {
+    const long long lo = s.first + i * s.keys - start, hi = lo + s.keys;
+    begin = lo <= 0 ? 0 : (lo >= len ? len : (int)lo / kSpanKeys * kSpanKeys);
+    end = hi <= 0 ? 0 : (hi >= len ? len : (int)hi / kSpanKeys * kSpanKeys);
+}
+#endif
+
+}  // namespace da

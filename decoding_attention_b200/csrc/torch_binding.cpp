@@ -8,6 +8,8 @@
 //   dmla_fwd(q, kv, cu_seq_k, max_seq_k, dim_v=512, is_alibi=False, softmax_scale=None, out=None, return_lse=False)
 //       the two named entry points with an explicit softmax scale; their defaults reproduce fwd().
 //   merge_partials(part_o, part_lse, out_dtype) -> (o, lse)           LSE merge of key-range shards.
+//   kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots=None), kv_cache_read(...) -> (k, v),
+//   quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, ...) -> o: caches with a scale per (token, KV head).
 //
 // Differences from the reference, all on the safe side: a device guard on q's device (the
 // reference takes none, so it only works on the current device), real row strides are passed down
@@ -239,6 +241,213 @@ std::tuple<at::Tensor, at::Tensor> merge_partials(const at::Tensor &part_o, cons
     return {o, lse};
 }
 
+// ---- caches of 8- and 4-bit codes with a scale per (token, KV head) ----------------------------
+struct QuantCache {
+    int32_t kv_dtype;
+    int64_t rows, head_k, dim, page_size;  // page_size 0: packed [rows, head_k, dim]
+};
+
+QuantCache check_cache(const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_scale, const at::Tensor &v_scale,
+                       const at::Device &device) {
+    QuantCache c;
+    switch (k.scalar_type()) {
+        case at::kFloat8_e4m3fn: c.kv_dtype = DA_KV_FP8_E4M3; break;
+        case at::kChar: c.kv_dtype = DA_KV_INT8; break;
+        case at::kByte: c.kv_dtype = DA_KV_INT4; break;
+        default: TORCH_CHECK(false, "k_cache must have dtype float8_e4m3fn, int8 or uint8 (two int4 codes a byte)");
+    }
+    TORCH_CHECK(v.dtype() == k.dtype(), "key and value caches must have the same dtype");
+    TORCH_CHECK(k_scale.dtype() == torch::kFloat32 && v_scale.dtype() == torch::kFloat32, "scales must have dtype float32");
+    for (const at::Tensor *t : {&k, &v, &k_scale, &v_scale}) {
+        TORCH_CHECK(t->is_cuda() && t->device() == device, "all tensors must be on one CUDA device");
+        TORCH_CHECK(t->is_contiguous(), "caches and scales must be contiguous");
+    }
+    TORCH_CHECK(k.dim() == 3 || k.dim() == 4, "k_cache must be [rows, head_k, dim] or [pages, page_size, head_k, dim]");
+    TORCH_CHECK(v.sizes() == k.sizes(), "k_cache and v_cache must have the same shape");
+    TORCH_CHECK(k_scale.sizes() == k.sizes().slice(0, k.dim() - 1) && v_scale.sizes() == k_scale.sizes(),
+                "scales must have the caches' shape without the last dimension");
+    c.page_size = k.dim() == 4 ? k.size(1) : 0;
+    c.rows = k.dim() == 4 ? k.size(0) * k.size(1) : k.size(0);
+    c.head_k = k.size(-2);
+    c.dim = k.size(-1) * (c.kv_dtype == DA_KV_INT4 ? 2 : 1);
+    return c;
+}
+
+void check_rows(const at::Tensor &x, const char *name, int64_t tokens, const QuantCache &c, const at::Device &device) {
+    TORCH_CHECK(x.is_cuda() && x.device() == device, "all tensors must be on one CUDA device");
+    TORCH_CHECK(x.dim() == 3 && x.size(0) == tokens && x.size(1) == c.head_k && x.size(2) == c.dim, name,
+                " must have shape (tokens, head_k, dim) with the caches' head_k and dim");
+    TORCH_CHECK(x.stride(2) == 1 && (c.head_k == 1 || x.stride(1) == c.dim), "heads must be contiguous inside a token row");
+}
+
+const int64_t *check_slots(const std::optional<at::Tensor> &slots, int64_t tokens, const at::Device &device) {
+    if (!slots.has_value()) return nullptr;
+    TORCH_CHECK(slots->is_cuda() && slots->device() == device, "all tensors must be on one CUDA device");
+    TORCH_CHECK(slots->dtype() == torch::kInt64 && slots->dim() == 1 && slots->size(0) == tokens && slots->is_contiguous(),
+                "slots must be a contiguous int64 tensor with one element per token");
+    return slots->data_ptr<int64_t>();
+}
+
+da_kv_rows_args_t rows_args(const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_cache, const at::Tensor &v_cache,
+                            const at::Tensor &k_scale, const at::Tensor &v_scale, const QuantCache &c) {
+    da_kv_rows_args_t a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.kv_dtype = c.kv_dtype;
+    a.x_dtype = k.scalar_type() == at::kHalf ? DA_ROWS_FP16 : (k.scalar_type() == at::kBFloat16 ? DA_ROWS_BF16 : DA_ROWS_FP32);
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    a.k_cache = k_cache.data_ptr();
+    a.v_cache = v_cache.data_ptr();
+    a.k_scale = k_scale.data_ptr<float>();
+    a.v_scale = v_scale.data_ptr<float>();
+    a.tokens = k.size(0);
+    a.cache_rows = c.rows;
+    a.head_k = c.head_k;
+    a.dim = c.dim;
+    // (a tensor of one token may carry any stride; the library wants one that covers the row)
+    a.k_row_stride = a.tokens > 1 ? k.stride(0) : 0;
+    a.v_row_stride = a.tokens > 1 ? v.stride(0) : 0;
+    a.stream = at::cuda::getCurrentCUDAStream().stream();
+    return a;
+}
+
+void kv_cache_write(const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_cache, const at::Tensor &v_cache,
+                    const at::Tensor &k_scale, const at::Tensor &v_scale, std::optional<at::Tensor> slots) {
+    TORCH_CHECK(k.dtype() == torch::kFloat16 || k.dtype() == torch::kBFloat16,
+                "Decoding-Attention only support FP16 and BF16 data type");
+    TORCH_CHECK(v.dtype() == k.dtype(), "key and value must have the same dtype");
+    const QuantCache c = check_cache(k_cache, v_cache, k_scale, v_scale, k.device());
+    TORCH_CHECK(k.dim() == 3, "key and value must be 3-D");
+    check_rows(k, "key", k.size(0), c, k.device());
+    check_rows(v, "value", k.size(0), c, k.device());
+    const at::cuda::CUDAGuard guard(k.device());
+    da_kv_rows_args_t a = rows_args(k, v, k_cache, v_cache, k_scale, v_scale, c);
+    a.slots = check_slots(slots, a.tokens, k.device());
+    const int rc = da_kv_cache_write(&a);
+    TORCH_CHECK(rc == DA_OK, "decoding_attn: ", da_status_string(rc), ": ", da_last_error());
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_cache_read(const at::Tensor &k_cache, const at::Tensor &v_cache,
+                                                 const at::Tensor &k_scale, const at::Tensor &v_scale,
+                                                 std::optional<at::Tensor> slots, at::ScalarType dtype,
+                                                 std::optional<std::tuple<at::Tensor, at::Tensor>> out) {
+    const at::Device device = k_cache.device();
+    const QuantCache c = check_cache(k_cache, v_cache, k_scale, v_scale, device);
+    TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16 || dtype == at::kFloat, "dtype must be float16, bfloat16 or float32");
+    const int64_t tokens = slots.has_value() ? slots->numel() : c.rows;
+    const at::cuda::CUDAGuard guard(device);
+    at::Tensor k, v;
+    if (out.has_value()) {
+        k = std::get<0>(*out);
+        v = std::get<1>(*out);
+        TORCH_CHECK(k.scalar_type() == dtype && v.scalar_type() == dtype, "Output must have the dtype asked for");
+        check_rows(k, "out[0]", tokens, c, device);
+        check_rows(v, "out[1]", tokens, c, device);
+    } else {
+        k = torch::empty({tokens, c.head_k, c.dim}, k_cache.options().dtype(dtype));
+        v = torch::empty({tokens, c.head_k, c.dim}, k_cache.options().dtype(dtype));
+    }
+    da_kv_rows_args_t a = rows_args(k, v, k_cache, v_cache, k_scale, v_scale, c);
+    a.slots = check_slots(slots, tokens, device);
+    const int rc = da_kv_cache_read(&a);
+    TORCH_CHECK(rc == DA_OK, "decoding_attn: ", da_status_string(rc), ": ", da_last_error());
+    return {k, v};
+}
+
+// q and the outputs of the decode calls below.
+void check_query(const at::Tensor &q, int64_t batch, int64_t head_k, int64_t dim) {
+    TORCH_CHECK(q.dtype() == torch::kFloat16 || q.dtype() == torch::kBFloat16,
+                "Decoding-Attention only support FP16 and BF16 data type");
+    DA_CHECK_DEVICE(q);
+    TORCH_CHECK(q.dim() == 3, "query must be 3-D");
+    TORCH_CHECK(batch > 0, "batch size must be positive");
+    TORCH_CHECK(q.size(0) == batch, "one query token per sequence: q.size(0) must equal cu_seq_k.numel() - 1");
+    TORCH_CHECK(q.size(2) == dim, "query and key must have the same head dim");
+    TORCH_CHECK(head_k > 0 && q.size(1) % head_k == 0, "number of heads in key/value must divide number of heads in query");
+    TORCH_CHECK(q.stride(2) == 1 && (q.size(1) == 1 || q.stride(1) == dim), "heads must be contiguous inside a token row");
+}
+Outputs make_outputs(const at::Tensor &q, const std::optional<at::Tensor> &out, bool want_lse) {
+    Outputs r;
+    if (out.has_value()) {
+        r.o = out.value();
+        TORCH_CHECK(r.o.dtype() == q.dtype(), "Output must have the same dtype as inputs");
+        TORCH_CHECK(r.o.is_cuda() && r.o.device() == q.device(), "all tensors must be on one device");
+        TORCH_CHECK(r.o.sizes() == q.sizes(), "out must have the shape of the query");
+        TORCH_CHECK(r.o.stride(2) == 1 && (q.size(1) == 1 || r.o.stride(1) == q.size(2)), "heads must be contiguous inside a token row");
+    } else {
+        r.o = torch::empty(q.sizes(), q.options());
+    }
+    if (want_lse) r.lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat32));
+    return r;
+}
+void check_cu(const at::Tensor &cu_seq_k, const at::Device &device) {
+    TORCH_CHECK(cu_seq_k.dtype() == torch::kInt32, "cu_seq_k must have dtype int32");
+    TORCH_CHECK(cu_seq_k.is_cuda() && cu_seq_k.device() == device, "all tensors must be on one device");
+    TORCH_CHECK(cu_seq_k.dim() == 1 && cu_seq_k.is_contiguous(), "cu_seq_k must be a contiguous 1-D tensor");
+}
+void check_table(const at::Tensor &table, int64_t batch, const at::Device &device) {
+    TORCH_CHECK(table.dtype() == torch::kInt32, "block_table must have dtype int32");
+    TORCH_CHECK(table.is_cuda() && table.device() == device, "all tensors must be on one device");
+    TORCH_CHECK(table.dim() == 2 && table.size(0) == batch && table.size(1) > 0 && (table.size(1) == 1 || table.stride(1) == 1),
+                "block_table must be [batch, blocks] with a contiguous last dimension");
+}
+int64_t row_stride(const at::Tensor &x) { return x.size(0) > 1 ? x.stride(0) : 0; }
+
+pybind11::object quantized_fwd(const at::Tensor &q, const at::Tensor &k_cache, const at::Tensor &v_cache,
+                               const at::Tensor &k_scale, const at::Tensor &v_scale, const at::Tensor &cu_seq_k,
+                               bool is_alibi, std::optional<double> softmax_scale, std::optional<at::Tensor> out,
+                               bool return_lse, std::optional<at::Tensor> block_table) {
+    const QuantCache c = check_cache(k_cache, v_cache, k_scale, v_scale, q.device());
+    check_cu(cu_seq_k, q.device());
+    const int64_t batch = cu_seq_k.numel() - 1;
+    check_query(q, batch, c.head_k, c.dim);
+    TORCH_CHECK(block_table.has_value() == (c.page_size > 0), "a paged cache (4-D) needs a block_table, a packed one takes none");
+    const at::cuda::CUDAGuard guard(q.device());
+    const Outputs r = make_outputs(q, out, return_lse);
+    da_quant_decode_args_t a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    a.is_bf16 = q.scalar_type() == at::kBFloat16;
+    a.is_alibi = is_alibi;
+    a.kv_dtype = c.kv_dtype;
+    a.q = q.data_ptr();
+    a.k = k_cache.data_ptr();
+    a.v = v_cache.data_ptr();
+    a.k_scale = k_scale.data_ptr<float>();
+    a.v_scale = v_scale.data_ptr<float>();
+    a.o = r.o.data_ptr();
+    a.lse = return_lse ? r.lse.data_ptr<float>() : nullptr;
+    a.cu_seq_k = cu_seq_k.data_ptr<int32_t>();
+    a.rows = c.rows;
+    a.batch = batch;
+    a.head_q = q.size(1);
+    a.head_k = c.head_k;
+    a.dim = c.dim;
+    a.q_row_stride = row_stride(q);
+    a.o_row_stride = row_stride(r.o);
+    if (block_table.has_value()) {
+        check_table(*block_table, batch, q.device());
+        a.block_table = block_table->data_ptr<int32_t>();
+        a.block_table_stride = batch > 1 ? block_table->stride(0) : block_table->size(1);
+        a.table_blocks = block_table->size(1);
+        a.page_size = (int32_t)c.page_size;
+    }
+    a.softmax_scale = softmax_scale.has_value() ? (float)softmax_scale.value() : 0.0f;
+    a.stream = at::cuda::getCurrentCUDAStream().stream();
+    const size_t bytes = da_quant_decode_workspace_bytes(&a);
+    at::Tensor workspace;
+    if (bytes > 0) {
+        workspace = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kUInt8));
+        a.workspace = workspace.data_ptr();
+        a.workspace_bytes = bytes;
+    }
+    const int rc = da_quant_decode_fwd(&a);
+    TORCH_CHECK(rc == DA_OK, "decoding_attn: ", da_status_string(rc), ": ", da_last_error());
+    if (return_lse) return pybind11::cast(std::make_tuple(r.o, r.lse));
+    return pybind11::cast(r.o);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -257,6 +466,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("softmax_scale") = py::none(), py::arg("out") = py::none(), py::arg("return_lse") = false);
     m.def("merge_partials", &merge_partials, "LSE merge of key-range partials", py::arg("part_o"),
           py::arg("part_lse"), py::arg("out_dtype"));
+    m.def("kv_cache_write", &kv_cache_write, "Quantise K and V rows into a cache", py::arg("k"), py::arg("v"),
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("slots") = py::none());
+    m.def("kv_cache_read", &kv_cache_read, "Rows of a quantised cache", py::arg("k_cache"), py::arg("v_cache"),
+          py::arg("k_scale"), py::arg("v_scale"), py::arg("slots"), py::arg("dtype"), py::arg("out") = py::none());
+    m.def("quantized_fwd", &quantized_fwd, "Decode over a cache with a scale per token and head", py::arg("q"),
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("cu_seq_k"),
+          py::arg("is_alibi") = false, py::arg("softmax_scale") = py::none(), py::arg("out") = py::none(),
+          py::arg("return_lse") = false, py::arg("block_table") = py::none());
     m.def("launch_count", []() { return da_launch_count(); });
     m.def("device_status", []() { return da_device_status(); });
 }

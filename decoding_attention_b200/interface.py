@@ -75,3 +75,44 @@ def paged_fwd(q, k_cache, v_cache, seq_lens, block_table, max_seq_k=None, dim_v=
 def merge_partials(part_o, part_lse, out_dtype):
     """LSE merge of partial results over disjoint key ranges: part_o fp32 [parts, ..., dim_v]."""
     return decoding_attn_cuda.merge_partials(part_o.contiguous(), part_lse.contiguous(), out_dtype)
+
+
+def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots=None):
+    """Quantise the rows of new tokens into a cache of 8- or 4-bit codes, one fp32 scale per (token, KV head).
+
+    k, v [tokens, head_k, dim], fp16 or bf16.  k_cache, v_cache: torch.float8_e4m3fn, torch.int8, or torch.uint8 for
+    int4 (two codes a byte, the even element in the low nibble, last dimension dim / 2); packed [rows, head_k, dim] or
+    paged [num_pages, page_size, head_k, dim]; dim 64, 96, 128 or 256.  k_scale, v_scale: float32 of that shape without
+    the last dimension.  ``slots`` (int64 [tokens]) names each token's cache row, ``page * page_size + offset`` in a
+    paged cache; a token whose slot is negative (padding) or past the cache is skipped, and two tokens of a call must
+    not name the same row.  Without ``slots`` token i goes to row i.  Written in place.
+
+    With a = max |x| of a row and Q = 448, 127 or 7: scale = a / Q, code = x * (Q / a) to the nearest, ties to even.
+    A row whose a is below 2^-100 becomes zeros, a row with an infinity or a NaN reads back as NaN.
+    The reference does not quantise its cache (README.md:154-156).
+    """
+    k, v = [maybe_contiguous(x) for x in (k, v)]
+    decoding_attn_cuda.kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+
+
+def kv_cache_read(k_cache, v_cache, k_scale, v_scale, slots=None, dtype=torch.bfloat16, out=None):
+    """The rows ``slots`` (int64 [tokens]; None: all of them, in order) of such a cache as (k, v) [tokens, head_k, dim].
+
+    ``dtype``: torch.float16, torch.bfloat16 or torch.float32; values are code * scale in fp32, rounded to it.  A slot that
+    is negative or past the cache gives a row of zeros.  ``out``: an optional pair of tensors to write to.
+    """
+    return decoding_attn_cuda.kv_cache_read(k_cache, v_cache, k_scale, v_scale, slots, dtype, out)
+
+
+def quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, is_alibi=False, softmax_scale=None, out=None,
+                  return_lse=False, block_table=None):
+    """Decode attention over a cache that ``kv_cache_write`` filled (any group size; dim 64, 96, 128 or 256).
+
+    q [batch, head_q, dim]; cu_seq_k int32 [batch + 1], cumulative lengths.  A packed cache holds key j of sequence b in
+    row ``cu_seq_k[b] + j``; a paged one (4-D, page_size a power of two) in row ``j % page_size`` of page
+    ``block_table[b, j // page_size]`` (int32).  Keys whose row or page lies outside the cache are masked.  No length hint
+    is needed: the work is divided on the device.  ``return_lse`` adds the fp32 natural-log LSE [batch, head_q].
+    """
+    q = maybe_contiguous(q)
+    return decoding_attn_cuda.quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, is_alibi, softmax_scale, out,
+                                            return_lse, block_table)

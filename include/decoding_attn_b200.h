@@ -185,6 +185,72 @@ int da_exchange_merge_bounded(const float *rec, void *const *peer_bufs, int32_t 
                               int32_t dim_v, uint32_t epoch, void *o, float *lse, int32_t is_bf16, void *stream,
                               int64_t max_wait_cycles);
 
+/* ---- Caches of 8- and 4-bit codes with a scale per (token, KV head) -------------------------------
+ * A cache row holds the codes of one token, [head_k, dim] (int4: two codes a byte, the element with the even
+ * index in the low nibble), and one fp32 scale per KV head; element = code * scale.  A paged pool
+ * [num_pages, page_size, head_k, dim] with scales [num_pages, page_size, head_k] is the same thing with
+ * num_pages * page_size rows.  None of the functions of this section has a counterpart in the reference, which lists
+ * KV-cache quantisation as not done (README.md:154-156). */
+
+enum { DA_ROWS_FP16 = 0, DA_ROWS_BF16 = 1, DA_ROWS_FP32 = 2 };
+
+/* Arguments of da_kv_cache_write / da_kv_cache_read.  Zero-initialise, set struct_size. */
+typedef struct da_kv_rows_args {
+    uint32_t struct_size;
+    int32_t kv_dtype; /* DA_KV_FP8_E4M3, DA_KV_INT8 or DA_KV_INT4 */
+    int32_t x_dtype;  /* type of k and v: DA_ROWS_FP16, DA_ROWS_BF16 or (reading only) DA_ROWS_FP32 */
+    int32_t reserved;
+    void *k, *v;               /* device [tokens, head_k, dim]: what is written, or where it is read to */
+    void *k_cache, *v_cache;   /* device [cache_rows, head_k, dim] codes */
+    float *k_scale, *v_scale;  /* device [cache_rows, head_k] */
+    const int64_t *slots;      /* device [tokens]: cache row of each token; NULL: row i for token i */
+    int64_t tokens, cache_rows, head_k, dim; /* dim: 64, 96, 128 or 256 */
+    int64_t k_row_stride, v_row_stride;      /* elements between tokens of k / v, 0 = packed */
+    void *stream;                            /* cudaStream_t */
+} da_kv_rows_args_t;
+
+/* Quantises k and v row by row (one token, one KV head) into the rows that `slots` names and stores the scales.  With
+ * a = max |x| of a row and Q = 448 (e4m3), 127 (int8) or 7 (int4): scale = a / Q rounded to fp32, code = x * (Q / a)
+ * with Q / a rounded to fp32 and the product rounded once, to nearest, ties to even.  A row with a < 2^-100 is stored as
+ * zeros with scale 0; a row that holds an infinity or a NaN gets scale NaN and codes 0.  A token whose slot is negative
+ * or not below cache_rows is skipped; all other cache rows stay as they are.  The slots of a call must differ: what
+ * a row named twice holds afterwards is unspecified. */
+int da_kv_cache_write(const da_kv_rows_args_t *args);
+/* k[i] = code * scale of row slots[i], the fp32 product rounded to x_dtype; the same for v.  A slot that is negative or
+ * not below cache_rows gives a row of zeros. */
+int da_kv_cache_read(const da_kv_rows_args_t *args);
+
+/* Arguments of da_quant_decode_fwd: da_decode_fwd's problem over such a cache.  Zero-initialise, set struct_size. */
+typedef struct da_quant_decode_args {
+    uint32_t struct_size;
+    int32_t is_bf16;  /* type of q and o: 0 fp16, 1 bf16 */
+    int32_t is_alibi; /* as in da_decode_args_t */
+    int32_t kv_dtype; /* DA_KV_FP8_E4M3, DA_KV_INT8 or DA_KV_INT4 */
+    const void *q;                  /* device [batch, head_q, dim] */
+    const void *k, *v;              /* device [rows, head_k, dim] codes, packed */
+    const float *k_scale, *v_scale; /* device [rows, head_k] */
+    void *o;                        /* device [batch, head_q, dim] */
+    float *lse;                     /* optional device [batch, head_q]: natural-log sum-exp of the scaled scores */
+    const int32_t *cu_seq_k;        /* device [batch + 1], cumulative lengths (not decreasing) */
+    int64_t rows;                   /* rows of the cache (pages * page_size): a key whose row is not below it is masked */
+    int64_t batch, head_q, head_k, dim; /* dim: 64, 96, 128 or 256; any group size */
+    int64_t q_row_stride, o_row_stride; /* in elements, 0 = packed */
+    const int32_t *block_table;     /* optional device [batch, block_table_stride]; NULL: key j of sequence b is row cu_seq_k[b] + j */
+    int64_t block_table_stride, table_blocks; /* elements per row, and how many of them are pages: keys behind them are masked */
+    int32_t page_size;              /* a power of two, with a block table */
+    float softmax_scale;            /* <= 0 selects 1/sqrt(dim) */
+    void *workspace;                /* device scratch of at least da_quant_decode_workspace_bytes() bytes */
+    size_t workspace_bytes;
+    void *stream;
+} da_quant_decode_args_t;
+
+/* o = softmax(scale * q . (k k_scale)^T + alibi) . (v v_scale) for one query token per sequence.  The work is cut by
+ * keys on the device, so no length hint is taken.  Codes are widened exactly; the softmax weights are rounded to 11
+ * bits, everything else is fp32.  A zero-length sequence, or one whose keys are all masked, gives a zero row and
+ * LSE = -inf.  The workspace needs no clearing; calls that may overlap need one each.  Graph-capturable. */
+int da_quant_decode_fwd(const da_quant_decode_args_t *args);
+size_t da_quant_decode_workspace_bytes(const da_quant_decode_args_t *args);
+
 /* Profiling hook for the calling thread: while both are non-NULL, da_decode_fwd records the CUDA
  * event `start_event` on the stream just before its main (key-streaming) kernel and `stop_event`
  * just after it, so a benchmark can time that kernel apart from the merge kernel.  Pass NULLs to
