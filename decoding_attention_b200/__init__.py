@@ -10,7 +10,7 @@ __version__ = "0.1.0"
 
 def __getattr__(name):
     if name in ("decoding_attn_fwd", "dmha_fwd", "dmla_fwd", "paged_fwd", "merge_partials", "kv_cache_write",
-                "kv_cache_read", "quantized_fwd"):
+                "kv_cache_read", "quantized_fwd", "shared_prefix_fwd"):
         from . import interface
         return getattr(interface, name)
     raise AttributeError(name)

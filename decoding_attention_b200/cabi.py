@@ -14,7 +14,7 @@ DA_OK, DA_ERR_INVALID_ARG, DA_ERR_UNSUPPORTED, DA_ERR_WORKSPACE, DA_ERR_CUDA, DA
 
 EXPORTS = ["da_decode_fwd", "da_decode_fwd_host", "da_decode_fwd_static", "da_static_scratch_bytes", "da_decode_workspace_bytes", "da_decode_num_splits", "da_plan_num_splits",
            "da_merge_partials", "da_exchange_merge", "da_exchange_merge_bounded", "da_exchange_buffer_bytes", "da_kv_cache_write", "da_kv_cache_read", "da_quant_decode_fwd",
-           "da_quant_decode_workspace_bytes", "da_set_profile_events", "da_selftest_wait_timeout", "da_device_status", "da_status_string", "da_last_error", "da_launch_count"]
+           "da_quant_decode_workspace_bytes", "da_prefix_decode_fwd", "da_prefix_decode_workspace_bytes", "da_set_profile_events", "da_selftest_wait_timeout", "da_device_status", "da_status_string", "da_last_error", "da_launch_count"]
 
 
 class DecodeArgs(ctypes.Structure):
@@ -62,6 +62,25 @@ class QuantDecodeArgs(ctypes.Structure):
         ("dim", ctypes.c_int64), ("q_row_stride", ctypes.c_int64), ("o_row_stride", ctypes.c_int64),
         ("block_table", ctypes.c_void_p), ("block_table_stride", ctypes.c_int64), ("table_blocks", ctypes.c_int64),
         ("page_size", ctypes.c_int32), ("softmax_scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class PrefixDecodeArgs(ctypes.Structure):
+    """Mirror of ``da_prefix_decode_args_t``."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("is_bf16", ctypes.c_int32), ("is_alibi", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("k_prefix", ctypes.c_void_p), ("v_prefix", ctypes.c_void_p), ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p), ("cu_seq_k", ctypes.c_void_p),
+        ("prefix_len", ctypes.c_int64), ("prefix_rows", ctypes.c_int64), ("rows", ctypes.c_int64), ("batch", ctypes.c_int64),
+        ("head_q", ctypes.c_int64), ("head_k", ctypes.c_int64), ("dim", ctypes.c_int64),
+        ("q_row_stride", ctypes.c_int64), ("o_row_stride", ctypes.c_int64), ("k_prefix_row_stride", ctypes.c_int64),
+        ("v_prefix_row_stride", ctypes.c_int64), ("k_row_stride", ctypes.c_int64), ("v_row_stride", ctypes.c_int64),
+        ("prefix_table", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("block_table_stride", ctypes.c_int64),
+        ("table_blocks", ctypes.c_int64), ("prefix_page_size", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float), ("reserved", ctypes.c_int32),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
     ]
 
@@ -115,6 +134,10 @@ def lib():
         l.da_quant_decode_fwd.argtypes = [ctypes.POINTER(QuantDecodeArgs)]
         l.da_quant_decode_workspace_bytes.restype = ctypes.c_size_t
         l.da_quant_decode_workspace_bytes.argtypes = [ctypes.POINTER(QuantDecodeArgs)]
+        l.da_prefix_decode_fwd.restype = ctypes.c_int
+        l.da_prefix_decode_fwd.argtypes = [ctypes.POINTER(PrefixDecodeArgs)]
+        l.da_prefix_decode_workspace_bytes.restype = ctypes.c_size_t
+        l.da_prefix_decode_workspace_bytes.argtypes = [ctypes.POINTER(PrefixDecodeArgs)]
         l.da_set_profile_events.restype = None
         l.da_set_profile_events.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         l.da_selftest_wait_timeout.restype = ctypes.c_int

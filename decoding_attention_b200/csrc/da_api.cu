@@ -172,6 +172,32 @@ EncodeTiledFn encode_tiled_fn() {
     return fn;
 }
 
+}  // namespace
+
+int encode_tensor_map(const void *base, int rank, const uint64_t *dims, const uint64_t *strides, const uint32_t *box,
+                      bool swizzle128, int dtype, CUtensorMap *out) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return fail(DA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint32_t estr[3] = {1, 1, 1};
+    cuuint64_t d[3], st[2];
+    cuuint32_t bx[3];
+    for (int i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        bx[i] = box[i];
+        if (i + 1 < rank) st[i] = strides[i];
+    }
+    const CUtensorMapDataType dt = dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                              : (dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+    CUresult r = fn(out, dt, (cuuint32_t)rank,
+                    const_cast<void *>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(DA_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return DA_OK;
+}
+
+namespace {
+
 // Rank-3 map over a K or V tensor seen as [rows][head_k][dim] with box {dim, 1, tile_keys}.  The
 // row extent is not known to the library (only cu_seq_k on the device is), so it is set to the
 // largest value a coordinate can take; the kernels use the map only for tiles that lie wholly
@@ -213,23 +239,8 @@ int make_tensor_map(const void *base, int rank, const uint64_t *dims, const uint
             return DA_OK;
         }
     }
-    EncodeTiledFn fn = encode_tiled_fn();
-    if (!fn) return fail(DA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint32_t estr[3] = {1, 1, 1};
-    cuuint64_t d[3], st[2];
-    cuuint32_t bx[3];
-    for (int i = 0; i < rank; ++i) {
-        d[i] = dims[i];
-        bx[i] = box[i];
-        if (i + 1 < rank) st[i] = strides[i];
-    }
-    const CUtensorMapDataType dt = dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                              : (dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
-    CUresult r = fn(out, dt, (cuuint32_t)rank,
-                    const_cast<void *>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(DA_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    const int rc = encode_tensor_map(base, rank, dims, strides, box, swizzle128, dtype, out);
+    if (rc != DA_OK) return rc;
     MapCacheEntry &slot = g_map_cache[g_map_next];
     g_map_next = (g_map_next + 1) % 8;
     slot.key = key;
@@ -237,7 +248,6 @@ int make_tensor_map(const void *base, int rank, const uint64_t *dims, const uint
     slot.valid = true;
     return DA_OK;
 }
-
 int make_kv_tensor_map(const void *base, long long row_stride, int head_k, int dim, int tile, int dtype,
                        CUtensorMap *out) {
     const uint64_t eb = dtype == 2 ? 1 : 2;

@@ -1,4 +1,5 @@
-// C ABI of the operators around a quantised cache: writing rows, reading them back, decode attention over them.
+// C ABI of the operators around a quantised cache -- writing rows, reading them back, decode attention over them -- and
+// of decode attention behind a shared prefix.
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -7,6 +8,7 @@
 #include "../../include/decoding_attn_b200.h"
 #include "da_internal.h"
 #include "da_kv_rows.h"
+#include "da_prefix.h"
 #include "da_stream.h"
 #include "da_stream_plan.h"
 
@@ -190,6 +192,126 @@ void fill_quant(const da_quant_decode_args_t *a, int sms, StreamParams *p) {
     plan_stream((int)a->dim, a->kv_dtype, sms, p);
 }
 
+int check_prefix_args(const da_prefix_decode_args_t *a) {
+    if (!a) return failf(DA_ERR_INVALID_ARG, "args is NULL");
+    if (a->struct_size != sizeof(*a))
+        return failf(DA_ERR_INVALID_ARG, "struct_size %u != sizeof(da_prefix_decode_args_t) %zu", a->struct_size, sizeof(*a));
+    if (a->kv_dtype != DA_KV_SAME_AS_Q && !quantised_kind(a->kv_dtype))
+        return failf(DA_ERR_INVALID_ARG, "kv_dtype %d: 0 (the type of q), 1 (FP8 e4m3), 2 (int8) or 3 (int4) expected", a->kv_dtype);
+    const bool quant = a->kv_dtype != DA_KV_SAME_AS_Q;
+    if (a->dim != 64 && a->dim != 96 && a->dim != 128) return failf(DA_ERR_UNSUPPORTED, "unsupported dim %lld: 64, 96 or 128", (long long)a->dim);
+    if (a->batch <= 0 || a->head_q <= 0 || a->head_k <= 0) return failf(DA_ERR_INVALID_ARG, "batch, head_q and head_k must be positive");
+    if (a->head_q % a->head_k != 0)
+        return failf(DA_ERR_INVALID_ARG, "head_q (%lld) must be a multiple of head_k (%lld)", (long long)a->head_q, (long long)a->head_k);
+    if (a->head_q / a->head_k > 128) return failf(DA_ERR_UNSUPPORTED, "more than 128 query heads per KV head");
+    if (a->batch > 65535 || a->head_q > 65535) return failf(DA_ERR_INVALID_ARG, "batch and head_q must be <= 65535");
+    if (a->prefix_len < 0 || a->prefix_len > (1 << 30)) return failf(DA_ERR_INVALID_ARG, "prefix_len must be in [0, 2^30]");
+    if (a->rows < 0 || a->rows > INT32_MAX || a->prefix_rows < 0 || a->prefix_rows > INT32_MAX)
+        return failf(DA_ERR_INVALID_ARG, "rows and prefix_rows must be in [0, 2^31)");
+    if (!a->q || !a->o || !a->cu_seq_k) return failf(DA_ERR_INVALID_ARG, "q, o and cu_seq_k must not be NULL");
+    if (a->prefix_len > 0 && (!a->k_prefix || !a->v_prefix)) return failf(DA_ERR_INVALID_ARG, "k_prefix and v_prefix must not be NULL");
+    if (a->rows > 0 && (!a->k || !a->v || (quant && (!a->k_scale || !a->v_scale))))
+        return failf(DA_ERR_INVALID_ARG, "k, v and, for a quantised cache, k_scale and v_scale must not be NULL");
+    if (!quant && (a->k_scale || a->v_scale)) return failf(DA_ERR_INVALID_ARG, "scales given for a cache that is not quantised");
+    if (((uintptr_t)a->q | (uintptr_t)a->k_prefix | (uintptr_t)a->v_prefix | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->o |
+         (uintptr_t)a->workspace) & 15u)
+        return failf(DA_ERR_INVALID_ARG, "q, k_prefix, v_prefix, k, v, o and workspace must be 16-byte aligned");
+    if (((uintptr_t)a->k_scale | (uintptr_t)a->v_scale | (uintptr_t)a->cu_seq_k | (uintptr_t)a->lse | (uintptr_t)a->block_table |
+         (uintptr_t)a->prefix_table) & 3u)
+        return failf(DA_ERR_INVALID_ARG, "scales, cu_seq_k, lse and tables must be 4-byte aligned");
+    const int64_t strides[6] = {a->q_row_stride, a->o_row_stride, a->k_prefix_row_stride, a->v_prefix_row_stride, a->k_row_stride, a->v_row_stride};
+    for (int i = 0; i < 6; ++i)
+        if (strides[i] != 0 && (strides[i] < (i < 2 ? a->head_q : a->head_k) * a->dim || strides[i] % 8 != 0 || (i >= 4 && quant)))
+            return failf(DA_ERR_INVALID_ARG, "row strides must be multiples of 16 bytes and cover a row; a quantised cache is packed");
+    if (a->prefix_table) {
+        if (a->prefix_page_size < 16 || (a->prefix_page_size & (a->prefix_page_size - 1)) != 0)
+            return failf(DA_ERR_UNSUPPORTED, "prefix_page_size %d: a paged prefix needs a power of two >= 16", a->prefix_page_size);
+    } else {
+        if (a->prefix_page_size != 0) return failf(DA_ERR_INVALID_ARG, "prefix_page_size given without a prefix_table");
+        if (a->prefix_len > a->prefix_rows) return failf(DA_ERR_INVALID_ARG, "prefix_len exceeds prefix_rows");
+    }
+    if (a->block_table) {
+        if (a->page_size < 1 || (a->page_size & (a->page_size - 1)) != 0)
+            return failf(DA_ERR_UNSUPPORTED, "page_size %d: paged caches need a power of two", a->page_size);
+        if (a->table_blocks <= 0 || a->table_blocks > INT32_MAX || a->block_table_stride < a->table_blocks)
+            return failf(DA_ERR_INVALID_ARG, "table_blocks must be positive and block_table_stride cover them");
+    } else if (a->page_size != 0 || a->table_blocks != 0 || a->block_table_stride != 0) {
+        return failf(DA_ERR_INVALID_ARG, "page_size, table_blocks or block_table_stride given without a block_table");
+    }
+    return DA_OK;
+}
+
+PrefixGrid plan_prefix(int sms, int batch, int head_k, int group, int prefix_len) {
+    PrefixGrid g;
+    memset(&g, 0, sizeof(g));
+    g.tile_seqs = 128 / group < batch ? 128 / group : batch;
+    g.row_tiles = (batch + g.tile_seqs - 1) / g.tile_seqs;
+    g.pairs = (g.row_tiles + 1) / 2;
+    g.key_tiles = (prefix_len + 127) / 128;
+    const int64_t total = (int64_t)head_k * g.pairs * g.key_tiles;
+    g.cta_tiles = (int)((total + sms - 1) / sms);
+    g.ctas = (int)((total + g.cta_tiles - 1) / g.cta_tiles);
+    // parts of a unit: the runs that touch it, twice where its streams share one row tile
+    const int runs = (g.key_tiles + g.cta_tiles - 2) / g.cta_tiles + 1;
+    g.max_parts = runs * (g.row_tiles % 2 ? 2 : 1);
+    return g;
+}
+
+struct PrefixPlan {
+    PrefixGrid grid;
+    size_t parts, own, pieces;  // floats of each area of the workspace, a multiple of 4
+    size_t bytes() const { return (parts + own + pieces) * sizeof(float); }
+};
+
+PrefixPlan fill_prefix(const da_prefix_decode_args_t *a, int sms, StreamParams *s) {
+    da_quant_decode_args_t d;  // the sequences' own keys are the other entry point's problem
+    memset(&d, 0, sizeof(d));
+    d.is_bf16 = a->is_bf16;
+    d.is_alibi = a->is_alibi;
+    d.kv_dtype = a->kv_dtype;
+    d.q = a->q;
+    d.k = a->k;
+    d.v = a->v;
+    d.k_scale = a->k_scale;
+    d.v_scale = a->v_scale;
+    d.o = a->o;
+    d.lse = a->lse;
+    d.cu_seq_k = a->cu_seq_k;
+    d.rows = a->rows;
+    d.batch = a->batch;
+    d.head_q = a->head_q;
+    d.head_k = a->head_k;
+    d.dim = a->dim;
+    d.q_row_stride = a->q_row_stride;
+    d.o_row_stride = a->o_row_stride;
+    d.block_table = a->block_table;
+    d.block_table_stride = a->block_table_stride;
+    d.table_blocks = a->table_blocks;
+    d.page_size = a->page_size;
+    d.softmax_scale = a->softmax_scale;
+    fill_quant(&d, sms, s);
+    if (a->k_row_stride) s->k_row_stride = a->k_row_stride;
+    if (a->v_row_stride) s->v_row_stride = a->v_row_stride;
+    const size_t rows = (size_t)a->batch * a->head_q, row = (size_t)a->dim + 1;
+    PrefixPlan plan;
+    memset(&plan, 0, sizeof(plan));
+    if (a->prefix_len > 0) {
+        plan.grid = plan_prefix(sms, s->batch, s->head_k, s->group, (int)a->prefix_len);
+        plan.parts = ((size_t)plan.grid.max_parts * rows * row + 3) / 4 * 4;
+        plan.own = (rows * row + 3) / 4 * 4;
+    }
+    plan.pieces = stream_piece_bytes(*s, (int)a->dim) / sizeof(float);
+    return plan;
+}
+
+// Row maps of a prefix: K or V as [rows][head_k][dim], 64 columns of a box of rows.
+int prefix_map(const void *base, int64_t rows, int64_t row_stride, int box_rows, const da_prefix_decode_args_t *a, CUtensorMap *out) {
+    const uint64_t dims[3] = {(uint64_t)a->dim, (uint64_t)a->head_k, (uint64_t)rows};
+    const uint64_t strides[2] = {(uint64_t)a->dim * 2, (uint64_t)row_stride * 2};
+    const uint32_t box[3] = {64, 1, (uint32_t)box_rows};
+    return encode_tensor_map(base, 3, dims, strides, box, true, a->is_bf16 ? 1 : 0, out);
+}
+
 }  // namespace
 }  // namespace da
 
@@ -228,6 +350,80 @@ int da_quant_decode_fwd(const da_quant_decode_args_t *a) {
     cudaError_t e = launch_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream, false);
     if (e == cudaSuccess) e = launch_stream_merge(m, stream, true);
     if (e != cudaSuccess) return failf(DA_ERR_CUDA, "decode kernel launch: %s", cudaGetErrorString(e));
+    return DA_OK;
+}
+
+size_t da_prefix_decode_workspace_bytes(const da_prefix_decode_args_t *a) {
+    int sms = 0;
+    if (check_prefix_args(a) != DA_OK || sm_count(&sms) != DA_OK) return 0;
+    StreamParams s;
+    return fill_prefix(a, sms, &s).bytes();
+}
+
+int da_prefix_decode_fwd(const da_prefix_decode_args_t *a) {
+    int sms = 0;
+    int rc = check_prefix_args(a);
+    if (rc == DA_OK) rc = sm_count(&sms);
+    if (rc != DA_OK) return rc;
+    StreamMergeParams m;
+    memset(&m, 0, sizeof(m));
+    const PrefixPlan plan = fill_prefix(a, sms, &m.s);
+    if (!a->workspace || a->workspace_bytes < plan.bytes())
+        return failf(DA_ERR_WORKSPACE, "workspace has %zu bytes, %zu needed", a->workspace ? a->workspace_bytes : (size_t)0, plan.bytes());
+    float *parts = static_cast<float *>(a->workspace);
+    const size_t rows = (size_t)a->batch * a->head_q;
+    m.s.part_o = parts + plan.parts + plan.own;
+    m.s.part_lse = m.s.part_o + (size_t)m.s.spans * 2 * m.s.head_q * a->dim;
+    m.dim = (int)a->dim;
+    m.o = a->o;
+    m.lse = a->lse;
+    cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+    cudaError_t e = cudaSuccess;
+    if (a->prefix_len > 0) {
+        PrefixParams p;
+        memset(&p, 0, sizeof(p));
+        p.grid = plan.grid;
+        p.k = a->k_prefix;
+        p.v = a->v_prefix;
+        p.table = a->prefix_table;
+        p.k_row_stride = a->k_prefix_row_stride ? a->k_prefix_row_stride : a->head_k * a->dim;
+        p.v_row_stride = a->v_prefix_row_stride ? a->v_prefix_row_stride : a->head_k * a->dim;
+        p.rows = a->prefix_table ? a->prefix_rows : a->prefix_len;
+        for (int ps = a->prefix_page_size; ps > 1; ps >>= 1) ++p.page_shift;
+        p.prefix_len = (int)a->prefix_len;
+        p.batch = m.s.batch;
+        p.head_q = m.s.head_q;
+        p.head_k = m.s.head_k;
+        p.group = m.s.group;
+        p.dim = (int)a->dim;
+        p.cu_seq_k = a->cu_seq_k;
+        p.is_alibi = m.s.is_alibi;
+        p.scale_log2 = m.s.scale_log2;
+        p.part_o = parts;
+        p.part_lse = parts + (size_t)plan.grid.max_parts * rows * a->dim;
+        rc = xmerge_status_ptr(&p.status);
+        CUtensorMap tm_q, tm_k, tm_v;
+        const int box = a->prefix_table && a->prefix_page_size < 128 ? a->prefix_page_size : 128;
+        const uint64_t qd[3] = {(uint64_t)a->dim, (uint64_t)a->head_q, (uint64_t)a->batch};
+        const uint64_t qs[2] = {(uint64_t)a->dim * 2, (uint64_t)m.s.q_row_stride * 2};
+        const uint32_t qb[3] = {64, (uint32_t)p.group, (uint32_t)plan.grid.tile_seqs};
+        if (rc == DA_OK) rc = encode_tensor_map(a->q, 3, qd, qs, qb, true, a->is_bf16 ? 1 : 0, &tm_q);
+        if (rc == DA_OK) rc = prefix_map(p.k, p.rows, p.k_row_stride, box, a, &tm_k);
+        if (rc == DA_OK) rc = prefix_map(p.v, p.rows, p.v_row_stride, box, a, &tm_v);
+        if (rc != DA_OK) return rc;
+        e = launch_prefix(a->is_bf16 != 0, p, tm_q, tm_k, tm_v, stream);
+        m.prefix_o = p.part_o;
+        m.prefix_lse = p.part_lse;
+        m.prefix = plan.grid;
+        m.s.o = nullptr;
+        m.s.lse = nullptr;
+        m.s.own_o = parts + plan.parts;
+        m.s.own_lse = m.s.own_o + rows * a->dim;
+        m.s.chained = 1;
+    }
+    if (e == cudaSuccess) e = launch_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream, m.s.chained != 0);
+    if (e == cudaSuccess) e = launch_stream_merge(m, stream, true);
+    if (e != cudaSuccess) return failf(DA_ERR_CUDA, "shared-prefix kernel launch: %s", cudaGetErrorString(e));
     return DA_OK;
 }
 

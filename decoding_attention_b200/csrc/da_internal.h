@@ -71,6 +71,13 @@ cudaError_t launch_order(const int *cu_seq_k, int batch, long long max_len, int 
 
 void count_launch(int n = 1);
 
+// Tiled tensor map over 16-bit (dtype 0 fp16, 1 bf16) or one-byte (2) elements; dims, strides and box innermost first,
+// strides in bytes for dimensions 1 and up (dimension 0 is contiguous).
+int encode_tensor_map(const void *base, int rank, const uint64_t *dims, const uint64_t *strides, const uint32_t *box,
+                      bool swizzle128, int dtype, CUtensorMap *out);
+// The current device's kernel status block (da_device_status).
+int xmerge_status_ptr(int **out);
+
 // Launches `kernel`.  With `overlap` the launch may begin while the preceding kernel of the stream is
 // still running (programmatic dependent launch); the kernel then calls pdl_wait() before it reads
 // anything that kernel wrote.

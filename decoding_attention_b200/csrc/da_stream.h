@@ -5,6 +5,8 @@
 
 #include <cstdint>
 
+#include "da_prefix.h"
+
 namespace da {
 
 // The keys of all sequences, laid end to end as cu_seq_k has them, are cut into `spans` equal spans, one per CTA
@@ -32,6 +34,9 @@ struct StreamParams {
     int spans, min_span;           // CTAs along the keys; no span is shorter than min_span keys
     int is_alibi, q_bf16;
     float scale_log2;              // softmax scale * log2(e)
+    // Launched while the prefix kernel still runs: the grid then ends only after that one has, so that whoever waits for
+    // this grid may read the other's results too.
+    int chained;
 };
 
 // kind: 0 the type of q, 1 FP8 e4m3, 2 int8, 3 int4.
@@ -48,11 +53,11 @@ cudaError_t launch_stream_d96(int kind, bool bf16, const StreamParams &p, cudaSt
 cudaError_t launch_stream_d128(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
 cudaError_t launch_stream_d256(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
 
-// o = softmax-weighted sum of a row's pieces: those of the key stream, and (shared prefix) `prefix_parts` more.
+// o = softmax-weighted sum of a row's pieces: those of the key stream and, with a shared prefix, its parts.
 struct StreamMergeParams {
     StreamParams s;
-    const float *prefix_o, *prefix_lse;  // [prefix_parts][batch][head_q][dim], [prefix_parts][batch][head_q]
-    int prefix_parts;
+    const float *prefix_o, *prefix_lse;  // [max_parts][batch][head_q][dim], [max_parts][batch][head_q]; NULL: no prefix
+    PrefixGrid prefix;
     int dim;
     void *o;      // [batch, head_q, dim], rows s.o_row_stride apart
     float *lse;   // optional [batch, head_q]

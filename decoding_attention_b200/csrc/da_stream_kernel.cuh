@@ -284,7 +284,10 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
     pdl_launch_dependents();
     const SpanPlan plan = span_plan(p);
     const long long span = blockIdx.x;
-    if (span * plan.keys >= plan.total) return;
+    if (span * plan.keys >= plan.total) {
+        if (p.chained) pdl_wait();
+        return;
+    }
 
     const int kpart = warp / p.head_warps;
     const int stream = blockIdx.y * p.head_warps + warp % p.head_warps;
@@ -678,6 +681,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                 }
         }
     }
+    if (p.chained) pdl_wait();
 }
 
 template <int KIND, int D, int NT>

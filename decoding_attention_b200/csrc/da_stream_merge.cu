@@ -39,20 +39,21 @@ __global__ void __launch_bounds__(kMergeWarps * 32) da_stream_merge_kernel(const
     }
     if (whole && p.s.o) return;  // the stream kernel has written it
     const int stream_parts = whole ? 1 : spans;
-    const int parts = p.prefix_parts + stream_parts;
+    const int prefix_parts = p.prefix_o ? prefix_parts_of(p.prefix, head / p.s.group, b) : 0;
+    const int parts = prefix_parts + stream_parts;
     auto part_lse = [&](int i) -> float {
-        if (i < p.prefix_parts) return p.prefix_lse[(long long)i * p.s.batch * p.s.head_q + row];
+        if (i < prefix_parts) return p.prefix_lse[(long long)i * p.s.batch * p.s.head_q + row];
         if (whole) return p.s.own_lse[row];
-        i -= p.prefix_parts;
+        i -= prefix_parts;
         int begin, end;
         span_piece(plan, first_span + i, start, len, begin, end);
         if (begin >= end) return -INFINITY;
         return p.s.part_lse[((first_span + i) * 2 + (begin == 0 ? 1 : 0)) * p.s.head_q + head];
     };
     auto part_o = [&](int i) -> const float * {
-        if (i < p.prefix_parts) return p.prefix_o + ((long long)i * p.s.batch * p.s.head_q + row) * D;
+        if (i < prefix_parts) return p.prefix_o + ((long long)i * p.s.batch * p.s.head_q + row) * D;
         if (whole) return p.s.own_o + row * D;
-        i -= p.prefix_parts;
+        i -= prefix_parts;
         int begin, end;
         span_piece(plan, first_span + i, start, len, begin, end);
         return p.s.part_o + (((first_span + i) * 2 + (begin == 0 ? 1 : 0)) * p.s.head_q + head) * D;

@@ -10,6 +10,7 @@
 //   merge_partials(part_o, part_lse, out_dtype) -> (o, lse)           LSE merge of key-range shards.
 //   kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots=None), kv_cache_read(...) -> (k, v),
 //   quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, ...) -> o: caches with a scale per (token, KV head).
+//   shared_prefix_fwd(q, k_prefix, v_prefix, k, v, cu_seq_k, ...) -> o: decode of a batch whose sequences share a prefix.
 //
 // Differences from the reference, all on the safe side: a device guard on q's device (the
 // reference takes none, so it only works on the current device), real row strides are passed down
@@ -448,6 +449,120 @@ pybind11::object quantized_fwd(const at::Tensor &q, const at::Tensor &k_cache, c
     return pybind11::cast(r.o);
 }
 
+pybind11::object shared_prefix_fwd(const at::Tensor &q, const std::optional<at::Tensor> &k_prefix_,
+                                   const std::optional<at::Tensor> &v_prefix_, const at::Tensor &k, const at::Tensor &v,
+                                   const at::Tensor &cu_seq_k, bool is_alibi, std::optional<double> softmax_scale,
+                                   std::optional<at::Tensor> out, bool return_lse, const std::optional<at::Tensor> &k_scale,
+                                   const std::optional<at::Tensor> &v_scale, const std::optional<at::Tensor> &block_table,
+                                   const std::optional<at::Tensor> &prefix_table, std::optional<int64_t> prefix_len) {
+    const at::Device device = q.device();
+    TORCH_CHECK(k_scale.has_value() == v_scale.has_value(), "k_scale and v_scale come together");
+    TORCH_CHECK(k_prefix_.has_value() == v_prefix_.has_value(), "k_prefix and v_prefix come together");
+    check_cu(cu_seq_k, device);
+    const int64_t batch = cu_seq_k.numel() - 1;
+    da_prefix_decode_args_t a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+
+    // the sequences' own keys: codes with scales, or rows of q's type, packed or in pages
+    int64_t page_size = 0;
+    if (k_scale.has_value()) {
+        const QuantCache c = check_cache(k, v, *k_scale, *v_scale, device);
+        a.kv_dtype = c.kv_dtype;
+        a.k_scale = k_scale->data_ptr<float>();
+        a.v_scale = v_scale->data_ptr<float>();
+        a.rows = c.rows;
+        a.head_k = c.head_k;
+        a.dim = c.dim;
+        page_size = c.page_size;
+    } else {
+        TORCH_CHECK(k.dtype() == q.dtype() && v.dtype() == q.dtype(), "query, key and value must have the same dtype");
+        TORCH_CHECK(k.is_cuda() && k.device() == device && v.is_cuda() && v.device() == device, "all tensors must be on one device");
+        TORCH_CHECK(k.dim() == 3 || k.dim() == 4, "key must be [total_k, head_k, dim] or [pages, page_size, head_k, dim]");
+        TORCH_CHECK(v.sizes() == k.sizes(), "key and value must have the same shape");
+        a.head_k = k.size(-2);
+        a.dim = k.size(-1);
+        if (k.dim() == 4) {
+            TORCH_CHECK(k.is_contiguous() && v.is_contiguous(), "a paged cache must be contiguous");
+            page_size = k.size(1);
+            a.rows = k.size(0) * page_size;
+        } else {
+            a.rows = k.size(0);
+            for (const at::Tensor *t : {&k, &v})
+                TORCH_CHECK(t->stride(2) == 1 && (a.head_k == 1 || t->stride(1) == a.dim), "heads must be contiguous inside a token row");
+            a.k_row_stride = row_stride(k);
+            a.v_row_stride = row_stride(v);
+        }
+    }
+    check_query(q, batch, a.head_k, a.dim);
+    TORCH_CHECK(block_table.has_value() == (page_size > 0), "a paged cache (4-D) needs a block_table, a packed one takes none");
+
+    // the prefix: rows of its own, or pages of a pool of its own or of the sequences'
+    TORCH_CHECK(k_prefix_.has_value() || prefix_table.has_value(), "k_prefix and v_prefix, or a prefix_table into k and v, must be given");
+    TORCH_CHECK(k_prefix_.has_value() || (page_size > 0 && !k_scale.has_value()), "a prefix in the sequences' own cache needs a paged cache in q's dtype");
+    const at::Tensor &kp = k_prefix_.has_value() ? *k_prefix_ : k;
+    const at::Tensor &vp = v_prefix_.has_value() ? *v_prefix_ : v;
+    TORCH_CHECK(kp.is_cuda() && kp.device() == device && vp.is_cuda() && vp.device() == device, "all tensors must be on one device");
+    TORCH_CHECK(kp.dtype() == q.dtype() && vp.dtype() == q.dtype(), "the prefix must have the dtype of the query");
+    TORCH_CHECK(kp.dim() == (prefix_table.has_value() ? 4 : 3), "the prefix must be [prefix_len, head_k, dim], or [pages, page_size, head_k, dim] with a prefix_table");
+    TORCH_CHECK(vp.sizes() == kp.sizes() && kp.size(-2) == a.head_k && kp.size(-1) == a.dim, "prefix and own keys must have the same head_k and dim");
+    if (prefix_table.has_value()) {
+        TORCH_CHECK(kp.is_contiguous() && vp.is_contiguous(), "a paged prefix must be contiguous");
+        TORCH_CHECK(prefix_table->dtype() == torch::kInt32 && prefix_table->dim() == 1 && prefix_table->is_contiguous(), "prefix_table must be a contiguous 1-D int32 tensor");
+        TORCH_CHECK(prefix_table->is_cuda() && prefix_table->device() == device, "all tensors must be on one device");
+        TORCH_CHECK(prefix_len.has_value(), "a paged prefix needs prefix_len");
+        a.prefix_len = *prefix_len;
+        a.prefix_page_size = (int32_t)kp.size(1);
+        a.prefix_rows = kp.size(0) * kp.size(1);
+        a.prefix_table = prefix_table->data_ptr<int32_t>();
+        TORCH_CHECK(a.prefix_len <= prefix_table->numel() * kp.size(1), "prefix_len exceeds the pages of prefix_table");
+    } else {
+        for (const at::Tensor *t : {&kp, &vp})
+            TORCH_CHECK(t->stride(2) == 1 && (a.head_k == 1 || t->stride(1) == a.dim), "heads must be contiguous inside a token row");
+        a.prefix_len = prefix_len.has_value() ? *prefix_len : kp.size(0);
+        a.prefix_rows = kp.size(0);
+        a.k_prefix_row_stride = row_stride(kp);
+        a.v_prefix_row_stride = row_stride(vp);
+    }
+
+    const at::cuda::CUDAGuard guard(device);
+    const Outputs r = make_outputs(q, out, return_lse);
+    a.is_bf16 = q.scalar_type() == at::kBFloat16;
+    a.is_alibi = is_alibi;
+    a.q = q.data_ptr();
+    a.k_prefix = kp.data_ptr();
+    a.v_prefix = vp.data_ptr();
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    a.o = r.o.data_ptr();
+    a.lse = return_lse ? r.lse.data_ptr<float>() : nullptr;
+    a.cu_seq_k = cu_seq_k.data_ptr<int32_t>();
+    a.batch = batch;
+    a.head_q = q.size(1);
+    a.q_row_stride = row_stride(q);
+    a.o_row_stride = row_stride(r.o);
+    if (block_table.has_value()) {
+        check_table(*block_table, batch, device);
+        a.block_table = block_table->data_ptr<int32_t>();
+        a.block_table_stride = batch > 1 ? block_table->stride(0) : block_table->size(1);
+        a.table_blocks = block_table->size(1);
+        a.page_size = (int32_t)page_size;
+    }
+    a.softmax_scale = softmax_scale.has_value() ? (float)softmax_scale.value() : 0.0f;
+    a.stream = at::cuda::getCurrentCUDAStream().stream();
+    const size_t bytes = da_prefix_decode_workspace_bytes(&a);
+    at::Tensor workspace;
+    if (bytes > 0) {
+        workspace = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kUInt8));
+        a.workspace = workspace.data_ptr();
+        a.workspace_bytes = bytes;
+    }
+    const int rc = da_prefix_decode_fwd(&a);
+    TORCH_CHECK(rc == DA_OK, "decoding_attn: ", da_status_string(rc), ": ", da_last_error());
+    if (return_lse) return pybind11::cast(std::make_tuple(r.o, r.lse));
+    return pybind11::cast(r.o);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -474,6 +589,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("cu_seq_k"),
           py::arg("is_alibi") = false, py::arg("softmax_scale") = py::none(), py::arg("out") = py::none(),
           py::arg("return_lse") = false, py::arg("block_table") = py::none());
+    m.def("shared_prefix_fwd", &shared_prefix_fwd, "Decode behind a prefix that the batch shares", py::arg("q"),
+          py::arg("k_prefix"), py::arg("v_prefix"), py::arg("k"), py::arg("v"), py::arg("cu_seq_k"),
+          py::arg("is_alibi") = false, py::arg("softmax_scale") = py::none(), py::arg("out") = py::none(),
+          py::arg("return_lse") = false, py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
+          py::arg("block_table") = py::none(), py::arg("prefix_table") = py::none(), py::arg("prefix_len") = py::none());
     m.def("launch_count", []() { return da_launch_count(); });
     m.def("device_status", []() { return da_device_status(); });
 }

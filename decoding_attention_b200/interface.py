@@ -116,3 +116,24 @@ def quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, is_alibi=Fals
     q = maybe_contiguous(q)
     return decoding_attn_cuda.quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, is_alibi, softmax_scale, out,
                                             return_lse, block_table)
+
+
+def shared_prefix_fwd(q, k_prefix, v_prefix, k, v, cu_seq_k, is_alibi=False, softmax_scale=None, out=None, return_lse=False,
+                      k_scale=None, v_scale=None, block_table=None, prefix_table=None, prefix_len=None):
+    """Decode attention of a batch whose sequences share their first keys, which are read once for all of them.
+
+    Sequence b attends to the prefix and then to its own keys ``cu_seq_k[b] .. cu_seq_k[b + 1]`` (int32 [batch + 1]; a
+    sequence may have none).  q [batch, head_q, dim], dim 64, 96 or 128, at most 128 query heads per KV head.
+
+    The prefix is k_prefix, v_prefix [prefix_len, head_k, dim] in q's dtype (``prefix_len`` may name fewer rows), or pages
+    ``prefix_table`` (int32 [blocks]) with ``prefix_len`` keys of a pool [num_pages, page_size, head_k, dim]: k_prefix and
+    v_prefix, or k and v themselves where those are None.  page_size: a power of two >= 16.
+    The own keys k, v are packed [total_k, head_k, dim] or paged with a ``block_table`` [batch, blocks], in q's dtype, or as
+    codes with ``k_scale``, ``v_scale`` as ``kv_cache_write`` leaves them.  ALiBi counts positions through the prefix.
+    ``return_lse`` adds the fp32 natural-log LSE [batch, head_q] over prefix and own keys.
+    """
+    q, k_prefix, v_prefix = [maybe_contiguous(x) for x in (q, k_prefix, v_prefix)]
+    if k_scale is None:
+        k, v = [maybe_contiguous(x) for x in (k, v)]
+    return decoding_attn_cuda.shared_prefix_fwd(q, k_prefix, v_prefix, k, v, cu_seq_k, is_alibi, softmax_scale, out, return_lse,
+                                                k_scale, v_scale, block_table, prefix_table, prefix_len)

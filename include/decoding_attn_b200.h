@@ -251,6 +251,46 @@ typedef struct da_quant_decode_args {
 int da_quant_decode_fwd(const da_quant_decode_args_t *args);
 size_t da_quant_decode_workspace_bytes(const da_quant_decode_args_t *args);
 
+/* Arguments of da_prefix_decode_fwd.  Zero-initialise, set struct_size. */
+typedef struct da_prefix_decode_args {
+    uint32_t struct_size;
+    int32_t is_bf16;  /* type of q, o, k_prefix and v_prefix: 0 fp16, 1 bf16 */
+    int32_t is_alibi; /* as in da_decode_args_t; positions run through the prefix and on through the sequence's own keys */
+    int32_t kv_dtype; /* the sequences' own keys: DA_KV_SAME_AS_Q, or codes as in da_quant_decode_args_t */
+    const void *q;                       /* device [batch, head_q, dim] */
+    const void *k_prefix, *v_prefix;     /* device [prefix_rows, head_k, dim]: key j of the prefix is row j, or see prefix_table */
+    const void *k, *v;                   /* device [rows, head_k, dim]: the sequences' own keys behind the prefix */
+    const float *k_scale, *v_scale;      /* device [rows, head_k], for codes only */
+    void *o;                             /* device [batch, head_q, dim] */
+    float *lse;                          /* optional device [batch, head_q] */
+    const int32_t *cu_seq_k;             /* device [batch + 1], cumulative lengths of the sequences' own keys */
+    int64_t prefix_len, prefix_rows;     /* keys of the prefix (0 to 2^30); rows of k_prefix and v_prefix */
+    int64_t rows;                        /* rows of k and v */
+    int64_t batch, head_q, head_k, dim;  /* dim: 64, 96 or 128; at most 128 query heads per KV head */
+    int64_t q_row_stride, o_row_stride, k_prefix_row_stride, v_prefix_row_stride; /* in elements, 0 = packed */
+    int64_t k_row_stride, v_row_stride;  /* the same; 0 for codes */
+    const int32_t *prefix_table;         /* optional device [ceil(prefix_len / prefix_page_size)]: pages of the prefix; an entry
+                                          * outside the pool reads as rows of zeros */
+    const int32_t *block_table;          /* optional, as in da_quant_decode_args_t, for the sequences' own keys */
+    int64_t block_table_stride, table_blocks;
+    int32_t prefix_page_size;            /* a power of two >= 16, with a prefix_table */
+    int32_t page_size;                   /* a power of two, with a block_table */
+    float softmax_scale;                 /* <= 0 selects 1/sqrt(dim) */
+    int32_t reserved;
+    void *workspace;                     /* device scratch of at least da_prefix_decode_workspace_bytes() bytes */
+    size_t workspace_bytes;
+    void *stream;
+} da_prefix_decode_args_t;
+
+/* Decode attention of a batch whose sequences share their first prefix_len keys: one query token per sequence over
+ * [prefix ; own keys].  The prefix is read once for the whole batch and multiplied on the tensor cores with the query
+ * heads of all sequences as rows; the own keys (of any lengths, zero included) follow as in da_quant_decode_fwd, and the
+ * results are joined.  Softmax weights are rounded to the type of q (own keys stored as codes: 11 bits), everything else
+ * is fp32.  With prefix_len = 0 and no own keys a row is zero and its LSE -inf.  The workspace needs no clearing; calls that
+ * may overlap need one each.  Graph-capturable.  The reference has no counterpart. */
+int da_prefix_decode_fwd(const da_prefix_decode_args_t *args);
+size_t da_prefix_decode_workspace_bytes(const da_prefix_decode_args_t *args);
+
 /* Profiling hook for the calling thread: while both are non-NULL, da_decode_fwd records the CUDA
  * event `start_event` on the stream just before its main (key-streaming) kernel and `stop_event`
  * just after it, so a benchmark can time that kernel apart from the merge kernel.  Pass NULLs to

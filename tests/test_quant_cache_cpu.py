@@ -15,7 +15,8 @@ PTR = 1 << 20  # an aligned address that nobody follows
 
 
 def test_ctypes_structs_match_c_layout(native_lib):
-    mirrors = {"da_kv_rows_args_t": native_lib.KvRowsArgs, "da_quant_decode_args_t": native_lib.QuantDecodeArgs}
+    mirrors = {"da_kv_rows_args_t": native_lib.KvRowsArgs, "da_quant_decode_args_t": native_lib.QuantDecodeArgs,
+               "da_prefix_decode_args_t": native_lib.PrefixDecodeArgs}
     body = "".join('printf("%%zu\\n", sizeof(%s));' % t + "".join('printf("%%zu\\n", offsetof(%s, %s));' % (t, f[0]) for f in m._fields_)
                    for t, m in mirrors.items())
     with tempfile.TemporaryDirectory() as d:
@@ -90,6 +91,39 @@ def test_decode_shapes_are_refused(native_lib):
     for change in ({"dim": 80}, {"dim": 576}, {**PAGED, "page_size": 0}, {**PAGED, "page_size": 24}):
         assert lib.da_quant_decode_fwd(ctypes.byref(quant_args(native_lib, **change))) == native_lib.DA_ERR_UNSUPPORTED
     assert lib.da_quant_decode_fwd(None) == native_lib.DA_ERR_INVALID_ARG
+
+
+def prefix_args(native_lib, **change):
+    a = native_lib.PrefixDecodeArgs(struct_size=ctypes.sizeof(native_lib.PrefixDecodeArgs), is_bf16=1, q=PTR, k_prefix=PTR, v_prefix=PTR,
+                                    k=PTR, v=PTR, o=PTR, cu_seq_k=PTR, prefix_len=50, prefix_rows=64, rows=100, batch=2, head_q=8,
+                                    head_k=2, dim=128, workspace=PTR, workspace_bytes=1 << 30)
+    for name, value in change.items():
+        setattr(a, name, value)
+    return a
+
+
+SCALES = {"kv_dtype": 2, "k_scale": PTR, "v_scale": PTR}
+
+
+@pytest.mark.parametrize("change", [
+    {"struct_size": 0}, {"kv_dtype": -1}, {"kv_dtype": 4}, {"kv_dtype": 2}, {"k_scale": PTR}, {**SCALES, "v_scale": None},
+    {"batch": 0}, {"batch": 65536}, {"head_q": 7}, {"head_k": 0}, {"prefix_len": -1}, {"prefix_len": (1 << 30) + 1},
+    {"prefix_len": 65}, {"rows": 1 << 31}, {"prefix_rows": 1 << 31}, {"q": None}, {"o": None}, {"cu_seq_k": None},
+    {"k_prefix": None}, {"v": None}, {"v_prefix": PTR + 8}, {"workspace": PTR + 4}, {"cu_seq_k": PTR + 2}, {"q_row_stride": 1028},
+    {"k_prefix_row_stride": 128}, {"v_row_stride": 260}, {**SCALES, "k_row_stride": 512}, {"prefix_page_size": 16},
+    {"page_size": 16}, {**PAGED, "table_blocks": 0}, {**PAGED, "block_table_stride": 3}])
+def test_prefix_arguments_are_refused(native_lib, change):
+    lib = native_lib.lib()
+    assert lib.da_prefix_decode_fwd(ctypes.byref(prefix_args(native_lib, **change))) == native_lib.DA_ERR_INVALID_ARG
+    assert lib.da_prefix_decode_workspace_bytes(ctypes.byref(prefix_args(native_lib, **change))) == 0
+
+
+def test_prefix_shapes_are_refused(native_lib):
+    lib = native_lib.lib()
+    for change in ({"dim": 256}, {"dim": 80}, {"head_q": 258}, {"prefix_table": PTR}, {"prefix_table": PTR, "prefix_page_size": 8},
+                   {"prefix_table": PTR, "prefix_page_size": 48}, {**PAGED, "page_size": 12}):
+        assert lib.da_prefix_decode_fwd(ctypes.byref(prefix_args(native_lib, **change))) == native_lib.DA_ERR_UNSUPPORTED
+    assert lib.da_prefix_decode_fwd(None) == native_lib.DA_ERR_INVALID_ARG
 
 
 @pytest.mark.parametrize("kind", ["fp8", "int8", "int4"])
