@@ -66,8 +66,10 @@ void plan_stream(int dim, int kind, int sms, StreamParams *p) {
     const int blocks = (streams + p->head_warps - 1) / p->head_warps;
     const int slots = sms * shape.ctas_per_sm;
     p->spans = slots > blocks ? slots / blocks : 1;
-    // A warp runs at least two or four tiles: below that its start costs more than its keys.
-    p->min_span = p->key_warps * 32 > 64 ? p->key_warps * 32 : 64;
+    // A piece of a sequence costs a CTA about as long as 16 keys of a warp, however short it is (its queries, the joining of
+    // its warps, its output); a CTA gets at least twice as much again to do.
+    p->piece_cost = 16 * p->key_warps;
+    p->min_span = 48 * p->key_warps;
 }
 
 size_t stream_piece_bytes(const StreamParams &p, int dim) {

@@ -9,8 +9,9 @@
 
 namespace da {
 
-// The keys of all sequences, laid end to end as cu_seq_k has them, are cut into `spans` equal spans, one per CTA
-// (and head block).  The cut between two spans falls on a multiple of kSpanKeys keys of its sequence.
+// The batch's work is an axis on which sequence b takes piece_cost + len(b) units: what a piece costs however short it is,
+// in keys, then its keys.  The axis is cut into `spans` equal spans, one per CTA (and head block); a cut falls on a multiple
+// of kSpanKeys keys of its sequence.
 constexpr int kSpanKeys = 32;
 
 struct StreamParams {
@@ -31,7 +32,8 @@ struct StreamParams {
     int batch, head_q, head_k, group;
     int chunks;                    // warps that share a KV head (each has up to 8 NT of its query heads)
     int head_warps, key_warps;     // a CTA's eight warps: so many (KV head, chunk) streams x so many parts of the keys
-    int spans, min_span;           // CTAs along the keys; no span is shorter than min_span keys
+    int spans, min_span;           // CTAs along the axis; no span is shorter than min_span units
+    int piece_cost;
     int is_alibi, q_bf16;
     float scale_log2;              // softmax scale * log2(e)
     // Launched while the prefix kernel still runs: the grid then ends only after that one has, so that whoever waits for
@@ -64,26 +66,32 @@ struct StreamMergeParams {
 };
 cudaError_t launch_stream_merge(const StreamMergeParams &p, cudaStream_t s, bool overlap);
 
-// The cut of the batch's keys into spans, the same in the stream kernel and in the merge.
+// The cut of the axis into spans, the same in the stream kernel and in the merge.
 struct SpanPlan {
-    long long first, total;  // cu_seq_k[0], keys of the batch
-    long long keys;          // of a span
+    long long units;  // of a span
+    long long total;  // of the batch
+    int first;        // cu_seq_k[0]
+    int cost;
 };
 #ifdef __CUDACC__
 __device__ __forceinline__ SpanPlan span_plan(const StreamParams &p) {
     SpanPlan s;
     s.first = p.cu_seq_k[0];
-    s.total = p.cu_seq_k[p.batch] - s.first;
-    if (s.total < 0) s.total = 0;
-    long long keys = (s.total + p.spans - 1) / p.spans;
-    if (keys < p.min_span) keys = p.min_span;
-    s.keys = (keys + kSpanKeys - 1) / kSpanKeys * kSpanKeys;
+    s.cost = p.piece_cost;
+    long long keys = (long long)p.cu_seq_k[p.batch] - s.first;
+    s.total = (keys > 0 ? keys : 0) + (long long)p.batch * s.cost;
+    long long units = (s.total + p.spans - 1) / p.spans;
+    if (units < p.min_span) units = p.min_span;
+    s.units = (units + kSpanKeys - 1) / kSpanKeys * kSpanKeys;
     return s;
 }
-// Keys [begin, end) that span i has of a sequence of `len` keys that starts at `start` on the common axis; the cuts are
-// moved down to a multiple of kSpanKeys keys of the sequence.
+// Where sequence b, whose keys start at cu, begins on the axis.
+__device__ __forceinline__ long long axis_start(const SpanPlan &s, int b, int cu) {
+    return (long long)cu - s.first + (long long)b * s.cost;
+}
+// Keys [begin, end) that span i has of a sequence of `len` keys that begins at `start` on the axis.
 __device__ __forceinline__ void span_piece(const SpanPlan &s, long long i, long long start, int len, int &begin, int &end) {
-    const long long lo = s.first + i * s.keys - start, hi = lo + s.keys;
+    const long long lo = i * s.units - start - s.cost, hi = lo + s.units;
     begin = lo <= 0 ? 0 : (lo >= len ? len : (int)lo / kSpanKeys * kSpanKeys);
     end = hi <= 0 ? 0 : (hi >= len ? len : (int)hi / kSpanKeys * kSpanKeys);
 }

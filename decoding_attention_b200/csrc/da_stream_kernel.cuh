@@ -243,23 +243,24 @@ struct PieceCursor {
         // from sequence b on, the first one with keys in the span; false behind the last
         for (; b < p.batch; ++b) {
             start = p.cu_seq_k[b];
-            if (start >= s.first + (span + 1) * s.keys) return false;
+            const long long at = axis_start(s, b, start);
+            if (at >= (span + 1) * s.units) return false;
             len = p.cu_seq_k[b + 1] - start;
             if (len <= 0) continue;
-            span_piece(s, span, start, len, begin, end);
+            span_piece(s, span, at, len, begin, end);
             if (begin < end) return true;
         }
         return false;
     }
 };
 
-// Largest b in [0, batch) with cu_seq_k[b] <= x, by the lanes of a warp together (0 if there is none).
-__device__ __forceinline__ int find_sequence(const int *cu, int batch, long long x, int lane) {
+// Largest b in [0, batch) that begins on the axis at or before x, by the lanes of a warp together (0 if there is none).
+__device__ __forceinline__ int find_sequence(const SpanPlan &s, const int *cu, int batch, long long x, int lane) {
     int lo = 0, n = batch;
     while (n > 1) {
         const int step = (n + 31) / 32;
         const int at = lane * step;
-        const unsigned hit = __ballot_sync(0xffffffffu, at < n && cu[lo + at] <= x);
+        const unsigned hit = __ballot_sync(0xffffffffu, at < n && axis_start(s, lo + at, cu[lo + at]) <= x);
         const int count = __popc(hit);
         const int off = count > 0 ? (count - 1) * step : 0;
         lo += off;
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
     pdl_launch_dependents();
     const SpanPlan plan = span_plan(p);
     const long long span = blockIdx.x;
-    if (span * plan.keys >= plan.total) {
+    if (span * plan.units >= plan.total) {
         if (p.chained) pdl_wait();
         return;
     }
@@ -304,19 +305,28 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
     const long long vstep = KIND == 3 ? p.v_row_stride / 2 : p.v_row_stride * (C::kQuant ? 1 : 2);
 
     PieceCursor con;
-    con.b = find_sequence(p.cu_seq_k, p.batch, plan.first + span * plan.keys, lane);
+    con.b = find_sequence(plan, p.cu_seq_k, p.batch, span * plan.units, lane);
     bool more = con.load(p, plan, span);
 
     // ---- producer side: tiles in the order in which this warp will want them ----
+    // Tiles that a piece has for this warp, and the first key of the i-th it takes.  With ALiBi the scores grow towards the
+    // end of a sequence: walked back to front, the first tiles set the reference maxima for the rest.
+    auto tiles_of = [&](const PieceCursor &x) {
+        const int keys = x.end - x.begin - kpart * TK;
+        return keys > 0 ? (keys + stride - 1) / stride : 0;
+    };
+    auto tile_key = [&](const PieceCursor &x, int i, int n) { return x.begin + kpart * TK + (p.is_alibi ? n - 1 - i : i) * stride; };
     PieceCursor pro = con;
     bool pro_more = more && !idle;
-    int pro_key = pro.begin + kpart * TK;
+    int pro_at = 0, pro_n = pro_more ? tiles_of(pro) : 0, pro_key = 0;
     auto settle = [&]() {  // moves on to a piece that has a tile for this warp
-        while (pro_more && pro_key >= pro.end) {
+        while (pro_more && pro_at >= pro_n) {
             ++pro.b;
             pro_more = pro.load(p, plan, span);
-            pro_key = pro.begin + kpart * TK;
+            pro_at = 0;
+            pro_n = pro_more ? tiles_of(pro) : 0;
         }
+        pro_key = tile_key(pro, pro_at, pro_n);
     };
     auto lookup = [&]() -> int {  // the cache row of key pro_key + lane, or -1
         const int key = pro_key + lane;
@@ -358,7 +368,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                 cp_async4(sc + TK + lane, p.v_scale + at, row >= 0 ? 4u : 0u);
             }
             fill = fill + 1 == STAGES ? 0 : fill + 1;
-            pro_key += stride;
+            ++pro_at;
             settle();
             row_next = lookup();
         }
@@ -381,23 +391,42 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                 const bool have = !idle && n * 8 + r < heads;
                 const uint16_t *row = static_cast<const uint16_t *>(p.q) + (long long)con.b * p.q_row_stride +
                                       (long long)(head0 + (have ? n * 8 + r : 0)) * D;
+                uint16_t h[C::KSTEPS][4];  // the lane's elements of the head's row, as the reduction steps want them
+#pragma unroll
+                for (int s = 0; s < C::KSTEPS; s += KIND == 3 ? 2 : 1) {
+                    const int word = KIND == 3 ? s >> 1 : (C::kQuant ? s : 2 * s);
+                    const uint16_t *src = row + word_offset<RB, 4>(word, c) * C::EPW / 4;
+                    uint32_t v[4] = {0, 0, 0, 0};
+                    if (have) {
+                        if (KIND == 3) {
+                            const uint4 y = *reinterpret_cast<const uint4 *>(src);
+                            v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+                        } else {
+                            const uint2 y = *reinterpret_cast<const uint2 *>(src);
+                            v[0] = y.x, v[1] = y.y;
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < (KIND == 3 ? 2 : 1); ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int el = pair_elem<KIND>(s + t, e >> 1, e & 1);
+                            h[s + t][e] = (uint16_t)(v[el >> 1] >> (16 * (el & 1)));
+                        }
+                }
                 float x[C::KSTEPS][4];
                 float top = 0.0f;
 #pragma unroll
-                for (int s = 0; s < C::KSTEPS; ++s) {
-                    const int word = KIND == 3 ? s >> 1 : (C::kQuant ? s : 2 * s);
-                    const int dim = word_offset<RB, 4>(word, c) * C::EPW / 4;
+                for (int s = 0; s < C::KSTEPS; ++s)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint16_t h = have ? row[dim + pair_elem<KIND>(s, e >> 1, e & 1)] : (uint16_t)0;
                         if (C::kQuant) {
-                            x[s][e] = p.q_bf16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+                            x[s][e] = p.q_bf16 ? __uint_as_float((uint32_t)h[s][e] << 16) : __half2float(__ushort_as_half(h[s][e]));
                             top = fmaxf(top, fabsf(x[s][e]));
                         } else {
-                            x[s][e] = __uint_as_float((uint32_t)h);
+                            x[s][e] = __uint_as_float((uint32_t)h[s][e]);
                         }
                     }
-                }
                 float up = 1.0f, f = p.scale_log2;
                 if (C::kQuant) {
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -440,7 +469,9 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[t][n][e] = 0.0f;
 
-        for (int key0 = con.begin + kpart * TK; !idle && key0 < con.end; key0 += stride) {
+        const int tiles = idle ? 0 : tiles_of(con);
+        for (int step = 0; step < tiles; ++step) {
+            const int key0 = tile_key(con, step, tiles);
             cp_async_wait<STAGES - 2>();
             __syncwarp();
             issue();
@@ -604,7 +635,9 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
 #pragma unroll
                 for (int t = 0; t < C::MTILES; ++t) acc[t][n][e] *= inv, acc[t][n][2 + e] *= inv;
             }
+        const int live = (con.end - con.begin + TK - 1) / TK;  // key parts that had a tile, if fewer than there are
         for (int half = p.key_warps / 2; half > 0; half /= 2) {
+            if (half >= live) continue;
             const int other = kpart >= half ? kpart - half : kpart;
             float *slot = merge + ((other * p.head_warps + warp % p.head_warps) * NT * 8) * C::kMergeRow;
             if (kpart >= half && kpart < 2 * half) {
@@ -657,18 +690,37 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                     uint16_t *dst16 = static_cast<uint16_t *>(p.o) + (long long)con.b * p.o_row_stride + (long long)(head0 + h) * D;
                     const bool to16 = whole && p.o;
 #pragma unroll
-                    for (int t = 0; t < C::MTILES; ++t)
+                    for (int w = 0; w < C::VW; ++w) {
+                        constexpr int kHalfWord = RB & 16;  // the last word has two bytes then
+                        const int n_el = kHalfWord && w == C::VW - 1 ? C::EPW / 2 : C::EPW;
+                        const int dim = word_offset<RB, 8>(w, r) * C::EPW / 4;
+                        float x[C::EPW];
 #pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const int el = 2 * t + g;
-                            const int dim = word_offset<RB, 8>(el / C::EPW, r) * C::EPW / 4 + el % C::EPW;
-                            const float x = acc[t][n][2 * g + e] * inv;
-                            if (to16) {
-                                dst16[dim] = p.q_bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
-                            } else {
-                                dst32[dim] = x;
-                            }
+                        for (int i = 0; i < C::EPW; ++i) {
+                            const int el = w * C::EPW + i;
+                            x[i] = el < D / 8 ? acc[el >> 1][n][2 * (el & 1) + e] * inv : 0.0f;
                         }
+                        if (to16) {
+                            uint32_t y[C::EPW / 2];
+#pragma unroll
+                            for (int i = 0; i < C::EPW / 2; ++i) {
+                                if (p.q_bf16) {
+                                    const __nv_bfloat162 z = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                                    y[i] = *reinterpret_cast<const uint32_t *>(&z);
+                                } else {
+                                    const __half2 z = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                                    y[i] = *reinterpret_cast<const uint32_t *>(&z);
+                                }
+                            }
+                            if (n_el == 8) *reinterpret_cast<uint4 *>(dst16 + dim) = make_uint4(y[0], y[1 % (C::EPW / 2)], y[2 % (C::EPW / 2)], y[3 % (C::EPW / 2)]);
+                            else if (n_el == 4) *reinterpret_cast<uint2 *>(dst16 + dim) = make_uint2(y[0], y[1 % (C::EPW / 2)]);
+                            else *reinterpret_cast<uint32_t *>(dst16 + dim) = y[0];
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < C::EPW / 2; ++i)
+                                if (2 * i < n_el) *reinterpret_cast<float2 *>(dst32 + dim + 2 * i) = make_float2(x[2 * i], x[2 * i + 1]);
+                        }
+                    }
                     if (r == 0) {
                         if (to16) {
                             if (p.lse) p.lse[row] = lse;
