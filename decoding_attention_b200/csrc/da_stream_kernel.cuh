@@ -81,6 +81,9 @@ __device__ __forceinline__ void cp_async4(void *dst_smem, const void *src_gmem, 
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst_smem)), "l"(src_gmem), "r"(src_bytes)
                  : "memory");
 }
+__device__ __forceinline__ void cp_async16_full(void *dst_smem, const void *src_gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst_smem)), "l"(src_gmem) : "memory");
+}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -328,9 +331,24 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
         }
         pro_key = tile_key(pro, pro_at, pro_n);
     };
-    auto lookup = [&]() -> int {  // the cache row of key pro_key + lane, or -1
+    // The first cache row of the next tile if all its keys are there, one row behind the other; -1 otherwise.
+    auto lookup = [&]() -> int {
+        if (!pro_more || pro_key + TK > pro.end) return -1;
+        long long row;
+        if (p.block_table) {
+            const int block = pro_key >> p.page_shift;
+            if ((1 << p.page_shift) < TK || block >= p.table_blocks) return -1;
+            const int page = p.block_table[(long long)pro.b * p.table_stride + block];
+            row = page < 0 ? -1 : ((long long)page << p.page_shift) + (pro_key & ((1 << p.page_shift) - 1));
+        } else {
+            row = (long long)pro.start + pro_key;
+        }
+        return row >= 0 && row + TK <= p.rows ? (int)row : -1;
+    };
+    // Any other tile: the cache row of key pro_key + lane, or -1 (behind the end, outside the table, the pool or the cache).
+    auto lookup_row = [&]() -> int {
         const int key = pro_key + lane;
-        if (!pro_more || lane >= TK || key >= pro.end) return -1;
+        if (lane >= TK || key >= pro.end) return -1;
         long long row;
         if (p.block_table) {
             const int block = key >> p.page_shift;
@@ -345,27 +363,61 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
     settle();
     int row_next = lookup();
     int fill = 0;
+    constexpr uint32_t kAllKeys = TK == 32 ? 0xffffffffu : (1u << TK) - 1u;
+    constexpr int kCopies = TK * C::CPR / 32;         // 16-byte copies of a lane for a K tile
+    const int row_l = lane / C::CPR, chunk_l = lane % C::CPR;
     auto issue = [&]() {
         if (pro_more) {
             uint8_t *stage = ring + fill * C::kStageBytes;
-            const unsigned valid = __ballot_sync(0xffffffffu, row_next >= 0);
-            if (lane == 0) masks[fill] = valid;
-            const long long row = row_next;
+            float *sc = reinterpret_cast<float *>(stage + 2 * TK * RB);
+            if (row_next >= 0) {
+                if (lane == 0) masks[fill] = kAllKeys;
+                const uint8_t *ks = kbase + (long long)row_next * kstep, *vs = vbase + (long long)row_next * vstep;
+                if (32 % C::CPR == 0) {
+                    // copy i takes the rows 32 / CPR further: the lane's place in them stays the same
+                    ks += (long long)row_l * kstep + chunk_l * 16;
+                    vs += (long long)row_l * vstep + chunk_l * 16;
+                    const long long ks_next = 32 / C::CPR * kstep, vs_next = 32 / C::CPR * vstep;
 #pragma unroll
-            for (int i = 0; i < TK * C::CPR / 32; ++i) {
-                const int idx = i * 32 + lane;
-                const int tr = idx / C::CPR, ch = idx - tr * C::CPR;
-                const int src = __shfl_sync(0xffffffffu, (int)row, tr);
-                const long long at = src >= 0 ? src : 0;
-                const uint32_t bytes = src >= 0 ? 16u : 0u;
-                cp_async16(stage + tr * RB + k_chunk<RB>(tr, ch) * 16, kbase + at * kstep + ch * 16, bytes);
-                cp_async16(stage + TK * RB + tr * RB + v_chunk<RB>(tr, ch) * 16, vbase + at * vstep + ch * 16, bytes);
-            }
-            if (C::kQuant && lane < TK) {
-                const long long at = (row >= 0 ? row : 0) * p.head_k + head_k;
-                float *sc = reinterpret_cast<float *>(stage + 2 * TK * RB);
-                cp_async4(sc + lane, p.k_scale + at, row >= 0 ? 4u : 0u);
-                cp_async4(sc + TK + lane, p.v_scale + at, row >= 0 ? 4u : 0u);
+                    for (int i = 0; i < kCopies; ++i) {
+                        const int tr = i * (32 / C::CPR) + row_l;
+                        cp_async16_full(stage + tr * RB + k_chunk<RB>(tr, chunk_l) * 16, ks);
+                        cp_async16_full(stage + TK * RB + tr * RB + v_chunk<RB>(tr, chunk_l) * 16, vs);
+                        ks += ks_next;
+                        vs += vs_next;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kCopies; ++i) {
+                        const int idx = i * 32 + lane;
+                        const int tr = idx / C::CPR, ch = idx - tr * C::CPR;
+                        cp_async16_full(stage + tr * RB + k_chunk<RB>(tr, ch) * 16, ks + (long long)tr * kstep + ch * 16);
+                        cp_async16_full(stage + TK * RB + tr * RB + v_chunk<RB>(tr, ch) * 16, vs + (long long)tr * vstep + ch * 16);
+                    }
+                }
+                if (C::kQuant && lane < TK) {
+                    const long long at = (long long)(row_next + lane) * p.head_k + head_k;
+                    cp_async4(sc + lane, p.k_scale + at, 4u);
+                    cp_async4(sc + TK + lane, p.v_scale + at, 4u);
+                }
+            } else {
+                const int row = lookup_row();
+                const unsigned valid = __ballot_sync(0xffffffffu, row >= 0);
+                if (lane == 0) masks[fill] = valid;
+#pragma unroll 1
+                for (int idx = lane; idx < TK * C::CPR; idx += 32) {
+                    const int tr = idx / C::CPR, ch = idx - tr * C::CPR;
+                    const int src = __shfl_sync(0xffffffffu, row, tr);
+                    const long long at = src >= 0 ? src : 0;
+                    const uint32_t bytes = src >= 0 ? 16u : 0u;
+                    cp_async16(stage + tr * RB + k_chunk<RB>(tr, ch) * 16, kbase + at * kstep + ch * 16, bytes);
+                    cp_async16(stage + TK * RB + tr * RB + v_chunk<RB>(tr, ch) * 16, vbase + at * vstep + ch * 16, bytes);
+                }
+                if (C::kQuant && lane < TK) {
+                    const long long at = (long long)(row >= 0 ? row : 0) * p.head_k + head_k;
+                    cp_async4(sc + lane, p.k_scale + at, row >= 0 ? 4u : 0u);
+                    cp_async4(sc + TK + lane, p.v_scale + at, row >= 0 ? 4u : 0u);
+                }
             }
             fill = fill + 1 == STAGES ? 0 : fill + 1;
             ++pro_at;
@@ -507,20 +559,44 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
             for (int t = 0; t < MT; ++t)
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
-                    const int j = t * 16 + g * 8 + key_r;
-                    const float ks = C::kQuant ? sc[j] : 1.0f;
-                    const float pos = (float)(key0 + j - (con.len - 1));
-                    const bool masked = !((valid >> j) & 1u);
+                    const float ks = C::kQuant ? sc[t * 16 + g * 8 + key_r] : 1.0f;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float x = s[t][n][2 * g + e] * (C::kQuant ? factor[n][e] * ks : factor[n][e]);
-                            if (p.is_alibi) x = fmaf(slope[n][e], pos, x);
-                            x = masked ? -INFINITY : x;
-                            s[t][n][2 * g + e] = x;
-                            raise |= x > m[n][e] + 8.0f;
-                        }
+                        for (int e = 0; e < 2; ++e) s[t][n][2 * g + e] *= C::kQuant ? factor[n][e] * ks : factor[n][e];
+                }
+            if (p.is_alibi) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const float pos = (float)(key0 + t * 16 + g * 8 + key_r - (con.len - 1));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) s[t][n][2 * g + e] = fmaf(slope[n][e], pos, s[t][n][2 * g + e]);
+                    }
+            }
+            if (valid != kAllKeys) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const bool masked = !((valid >> (t * 16 + g * 8 + key_r)) & 1u);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) s[t][n][2 * g + e] = masked ? -INFINITY : s[t][n][2 * g + e];
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = s[0][n][e];
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) top = fmaxf(top, fmaxf(s[t][n][e], s[t][n][2 + e]));
+                    raise |= top > m[n][e] + 8.0f;
                 }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
