@@ -349,7 +349,7 @@ int da_quant_decode_fwd(const da_quant_decode_args_t *a) {
     m.o = a->o;
     m.lse = a->lse;
     cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
-    cudaError_t e = launch_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream, false);
+    cudaError_t e = launch_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream, true);
     if (e == cudaSuccess) e = launch_stream_merge(m, stream, true);
     if (e != cudaSuccess) return failf(DA_ERR_CUDA, "decode kernel launch: %s", cudaGetErrorString(e));
     return DA_OK;
@@ -423,7 +423,7 @@ int da_prefix_decode_fwd(const da_prefix_decode_args_t *a) {
         m.s.own_lse = m.s.own_o + rows * a->dim;
         m.s.chained = 1;
     }
-    if (e == cudaSuccess) e = launch_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream, m.s.chained != 0);
+    if (e == cudaSuccess) e = launch_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream, true);
     if (e == cudaSuccess) e = launch_stream_merge(m, stream, true);
     if (e != cudaSuccess) return failf(DA_ERR_CUDA, "shared-prefix kernel launch: %s", cudaGetErrorString(e));
     return DA_OK;

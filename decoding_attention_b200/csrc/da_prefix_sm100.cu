@@ -83,8 +83,6 @@ da_prefix_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap tm_q,
     using C = PrefixCfg<D>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    pdl_launch_dependents();
-
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t *q_s = smem, *slot_s = smem + C::kOffSlots;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
@@ -115,6 +113,8 @@ da_prefix_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap tm_q,
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    pdl_wait();  // the kernel before this call's may still be running
+    pdl_launch_dependents();
 
     const PrefixGrid g = p.grid;
     const long long total = (long long)p.head_k * g.pairs * g.key_tiles;
@@ -417,7 +417,7 @@ cudaError_t launch_typed(const PrefixParams &p, const CUtensorMap &tm_q, const C
         if (dev < 64) ready |= 1ull << dev;
     }
     count_launch();
-    return launch_kernel(da_prefix_kernel<T, D>, dim3(p.grid.ctas), kThreads, C::kSmemBytes, s, false, p, tm_q, tm_k, tm_v);
+    return launch_kernel(da_prefix_kernel<T, D>, dim3(p.grid.ctas), kThreads, C::kSmemBytes, s, true, p, tm_q, tm_k, tm_v);
 }
 
 }  // namespace

@@ -74,13 +74,17 @@ struct SpanPlan {
     int cost;
 };
 #ifdef __CUDACC__
+// a / b of positions on the axis, which nearly always fit 32 bits (a 64-bit division takes ten times as long).
+__device__ __forceinline__ long long axis_div(long long a, long long b) {
+    return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
 __device__ __forceinline__ SpanPlan span_plan(const StreamParams &p) {
     SpanPlan s;
     s.first = p.cu_seq_k[0];
     s.cost = p.piece_cost;
-    long long keys = (long long)p.cu_seq_k[p.batch] - s.first;
+    const long long keys = (long long)p.cu_seq_k[p.batch] - s.first;
     s.total = (keys > 0 ? keys : 0) + (long long)p.batch * s.cost;
-    long long units = (s.total + p.spans - 1) / p.spans;
+    long long units = axis_div(s.total + p.spans - 1, p.spans);
     if (units < p.min_span) units = p.min_span;
     s.units = (units + kSpanKeys - 1) / kSpanKeys * kSpanKeys;
     return s;

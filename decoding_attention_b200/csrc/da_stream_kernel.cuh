@@ -285,6 +285,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
     uint32_t *masks = reinterpret_cast<uint32_t *>(smem + kStreamWarps * STAGES * C::kStageBytes) + warp * STAGES;
     float *merge = reinterpret_cast<float *>(smem + kStreamWarps * STAGES * (C::kStageBytes + 4));
 
+    if (!p.chained) pdl_wait();  // the kernel before this call's may still be running
     pdl_launch_dependents();
     const SpanPlan plan = span_plan(p);
     const long long span = blockIdx.x;
