@@ -127,6 +127,7 @@ int run_rows(const da_kv_rows_args_t *a, bool write) {
     p.cache_rows = a->cache_rows;
     p.rows = (uint32_t)(a->tokens * a->head_k);
     p.head_k = (int)a->head_k;
+    p.by_heads = make_fast_div((uint32_t)a->head_k);
     const cudaError_t e = launch_kv_rows(p, (int)a->dim, a->x_dtype, a->kv_dtype, write, static_cast<cudaStream_t>(a->stream));
     if (e != cudaSuccess) return failf(DA_ERR_CUDA, "cache row kernel launch: %s", cudaGetErrorString(e));
     return DA_OK;

@@ -10,9 +10,11 @@
 // whatever reads it sees NaN.
 //
 // Bound: HBM.  A row costs 2D bytes on the 16-bit side and D (or D / 2) + 4 on the other; nothing is read twice.
-// A row belongs to L lanes of one warp that hold 8 values a piece (16-byte accesses on the 16-bit side), the maximum
-// is joined by xor shuffles inside these lanes, and a thread has kRows rows in flight, since the slot, the row
-// and (reading) the scale are a chain of two loads.
+// A row belongs to L = D / 16 lanes that hold two pieces of 8 values (16-byte accesses on the 16-bit side, lanes side by
+// side); a thread has kRows rows in flight, since the slot, the row and (reading) the scale are a chain of two loads.
+// Writing is close to the issue limit, so what is done once a row is done for kRows rows at a time: the maxima of four
+// rows are joined by reduce-scatter (five shuffles for L = 8 where four xor reductions take twelve), after which every
+// lane has the maximum of one row and the two quotients are worked out once for all of them.
 #include "da_internal.h"
 #include "da_kv_rows.h"
 
@@ -24,9 +26,11 @@ constexpr int kThreads = 256;
 // Lanes of a row and 8-value chunks of a lane.
 template <int D>
 struct RowCfg {
-    static constexpr int kLanes = D == 96 ? 4 : D / 8;
+    static constexpr int kLanes = D == 96 ? 4 : D / 16;
     static constexpr int kChunks = D / 8 / kLanes;
 };
+
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv &d) { return (__umulhi(n, d.mul) + n) >> d.shift; }
 
 template <int KVQ>
 __device__ __forceinline__ constexpr float code_max() {
@@ -74,69 +78,111 @@ __device__ __forceinline__ void store_codes(uint8_t *dst, const float (&x)[8], f
     }
 }
 
+// The larger 16-bit magnitude of each half, sign bits cleared: magnitudes compare as integers, and infinities and NaN come
+// out above every number.
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ float magnitude(uint32_t bits);
+template <>
+__device__ __forceinline__ float magnitude<__half>(uint32_t bits) {
+    return __half2float(__ushort_as_half((unsigned short)bits));
+}
+template <>
+__device__ __forceinline__ float magnitude<__nv_bfloat16>(uint32_t bits) {
+    return __uint_as_float(bits << 16);
+}
+
 // blockIdx.y: 0 the K rows, 1 the V rows.  Row r = token * head_k + head.
 template <typename T, int D, int KVQ, int kRows>
 __global__ void __launch_bounds__(kThreads) da_kv_write_kernel(const KvRowsParams p) {
     using C = RowCfg<D>;
+    constexpr int L = C::kLanes;
     constexpr int kRowBytes = KVQ == 3 ? D / 2 : D;
-    constexpr int kBlockRows = kThreads / C::kLanes;
+    constexpr int kBlockRows = kThreads / L;
+    static_assert(kRows == 1 || kRows == 4, "rows of a thread");
     const T *__restrict__ src = static_cast<const T *>(blockIdx.y ? p.v : p.k);
     const long long src_stride = blockIdx.y ? p.v_row_stride : p.k_row_stride;
     uint8_t *__restrict__ cache = static_cast<uint8_t *>(blockIdx.y ? p.v_cache : p.k_cache);
     float *__restrict__ scales = blockIdx.y ? p.v_scale : p.k_scale;
-    const int lane = threadIdx.x % C::kLanes;
-    const uint32_t total = p.rows;
-    const uint32_t first = blockIdx.x * (uint32_t)(kBlockRows * kRows) + threadIdx.x / C::kLanes;
-    const unsigned group = C::kLanes == 32 ? 0xffffffffu
-                                           : ((1u << (C::kLanes & 31)) - 1u) << ((threadIdx.x & 31) / C::kLanes * C::kLanes);
+    pdl_wait();  // the kernel before this one may still be running
+    pdl_launch_dependents();
+    const int lane = threadIdx.x % L;
+    const uint32_t first = blockIdx.x * (uint32_t)(kBlockRows * kRows) + threadIdx.x / L;
 
     uint4 raw[kRows][C::kChunks];
-    long long slot[kRows];
-    uint32_t head[kRows];
+    long long dst[kRows];  // row of the cache, or -1
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const uint32_t r = first + i * kBlockRows;
-        slot[i] = -1;
-        head[i] = 0;
-        if (r < total) {
-            const uint32_t token = r / (uint32_t)p.head_k;
-            head[i] = r - token * (uint32_t)p.head_k;
-            slot[i] = p.slots ? p.slots[token] : (long long)token;
-            const T *row = src + (long long)token * src_stride + (long long)head[i] * D;
+        dst[i] = -1;
 #pragma unroll
-            for (int c = 0; c < C::kChunks; ++c) raw[i][c] = __ldcs(reinterpret_cast<const uint4 *>(row) + lane + c * C::kLanes);
+        for (int c = 0; c < C::kChunks; ++c) raw[i][c] = make_uint4(0, 0, 0, 0);
+        if (r < p.rows) {
+            const uint32_t token = fast_div(r, p.by_heads), head = r - token * (uint32_t)p.head_k;
+            const long long slot = p.slots ? p.slots[token] : (long long)token;
+            const T *row = src + (long long)token * src_stride + (long long)head * D;
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c) raw[i][c] = __ldcs(reinterpret_cast<const uint4 *>(row) + lane + c * L);
+            if (slot >= 0 && slot < p.cache_rows) dst[i] = slot * p.head_k + head;
         }
     }
+    uint32_t top[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-        if (slot[i] < 0 || slot[i] >= p.cache_rows) continue;  // uniform over the lanes of a row
-        float x[C::kChunks][8];
-        uint32_t top = 0;  // the magnitudes compare as integers; infinities and NaN come out above every number
+        uint32_t t = 0;
 #pragma unroll
         for (int c = 0; c < C::kChunks; ++c) {
-            unpack8<T>(raw[i][c], x[c]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[c][e]) & 0x7fffffffu);
+            const uint4 &x = raw[i][c];
+            const uint32_t m = 0x7fff7fffu;
+            t = max_magnitude(t, max_magnitude(max_magnitude(x.x & m, x.y & m), max_magnitude(x.z & m, x.w & m)));
         }
+        top[i] = t;
+    }
+    // Lane q of a row's lanes comes to hold row `mine` = the top two bits of q (all rows of the one there is).
+    uint32_t t = top[0];
+    int mine = 0;
+    if (kRows == 4) {
+        const bool up = lane & (L / 2), up2 = lane & (L / 4);
+        const uint32_t give0 = up ? top[0] : top[2 % kRows], give1 = up ? top[1 % kRows] : top[3 % kRows];
+        const uint32_t keep0 = up ? top[2 % kRows] : top[0], keep1 = up ? top[3 % kRows] : top[1 % kRows];
+        const uint32_t a = max_magnitude(keep0, __shfl_xor_sync(0xffffffffu, give0, L / 2));
+        const uint32_t b = max_magnitude(keep1, __shfl_xor_sync(0xffffffffu, give1, L / 2));
+        t = max_magnitude(up2 ? b : a, __shfl_xor_sync(0xffffffffu, up2 ? a : b, L / 4));
+        mine = (up ? 2 : 0) + (up2 ? 1 : 0);
 #pragma unroll
-        for (int d = 1; d < C::kLanes; d <<= 1) top = max(top, __shfl_xor_sync(group, top, d));
-        const float amax = __uint_as_float(top);
-        float scale = 0.0f, inv = 0.0f;
-        if (top >= 0x7f800000u) {
-            scale = __uint_as_float(0x7fffffffu);
+        for (int d = L / 8; d > 0; d >>= 1) t = max_magnitude(t, __shfl_xor_sync(0xffffffffu, t, d));
+    } else {
 #pragma unroll
-            for (int c = 0; c < C::kChunks; ++c)
+        for (int d = L / 2; d > 0; d >>= 1) t = max_magnitude(t, __shfl_xor_sync(0xffffffffu, t, d));
+    }
+    const float amax = magnitude<T>(max(t & 0xffffu, t >> 16));
+    float scale = 0.0f, inv = 0.0f;
+    if (!(amax <= 3.4028235e38f)) {  // an infinity or a NaN
+        scale = inv = __uint_as_float(0x7fffffffu);
+    } else if (amax >= 7.8886091e-31f) {  // 2^-100
+        scale = __fdiv_rn(amax, code_max<KVQ>());
+        inv = __fdiv_rn(code_max<KVQ>(), amax);
+    }
+    long long own = dst[0];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[c][e] = 0.0f;
-        } else if (top >= 0x0d800000u) {  // 2^-100
-            scale = __fdiv_rn(amax, code_max<KVQ>());
-            inv = __fdiv_rn(code_max<KVQ>(), amax);
+    for (int i = 1; i < kRows; ++i) own = mine == i ? dst[i] : own;
+    if (own >= 0 && (lane & (kRows == 4 ? L / 4 - 1 : L - 1)) == 0) scales[own] = scale;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        float f = __shfl_sync(0xffffffffu, inv, kRows == 4 ? i * (L / 4) : 0, L);
+        const bool odd = f != f;
+        if (dst[i] < 0) continue;
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c) {
+            if (odd) raw[i][c] = make_uint4(0, 0, 0, 0);
+            float x[8];
+            unpack8<T>(raw[i][c], x);
+            store_codes<KVQ>(cache + dst[i] * kRowBytes + (lane + c * L) * (KVQ == 3 ? 4 : 8), x, odd ? 0.0f : f);
         }
-        const long long row = slot[i] * p.head_k + head[i];
-#pragma unroll
-        for (int c = 0; c < C::kChunks; ++c)
-            store_codes<KVQ>(cache + row * kRowBytes + (lane + c * C::kLanes) * (KVQ == 3 ? 4 : 8), x[c], inv);
-        if (lane == 0) scales[row] = scale;
     }
 }
 
@@ -163,6 +209,8 @@ __global__ void __launch_bounds__(kThreads) da_kv_read_kernel(const KvRowsParams
     const long long dst_stride = blockIdx.y ? p.v_row_stride : p.k_row_stride;
     const uint8_t *__restrict__ cache = static_cast<const uint8_t *>(blockIdx.y ? p.v_cache : p.k_cache);
     const float *__restrict__ scales = blockIdx.y ? p.v_scale : p.k_scale;
+    pdl_wait();
+    pdl_launch_dependents();
     const int lane = threadIdx.x % C::kLanes;
     const uint32_t total = p.rows;
     const uint32_t first = blockIdx.x * (uint32_t)(kBlockRows * kRows) + threadIdx.x / C::kLanes;
@@ -170,10 +218,12 @@ __global__ void __launch_bounds__(kThreads) da_kv_read_kernel(const KvRowsParams
     uint2 raw[kRows][C::kChunks];
     float scale[kRows];
     long long slot[kRows];
+    uint32_t token[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const uint32_t r = first + i * kBlockRows;
-        slot[i] = r < total ? (p.slots ? p.slots[r / (uint32_t)p.head_k] : (long long)(r / (uint32_t)p.head_k)) : -1;
+        token[i] = fast_div(r < total ? r : 0, p.by_heads);
+        slot[i] = r < total ? (p.slots ? p.slots[token[i]] : (long long)token[i]) : -1;
     }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
@@ -182,7 +232,7 @@ __global__ void __launch_bounds__(kThreads) da_kv_read_kernel(const KvRowsParams
         for (int c = 0; c < C::kChunks; ++c) raw[i][c] = make_uint2(0, 0);
         if (slot[i] < 0 || slot[i] >= p.cache_rows) continue;
         const uint32_t r = first + i * kBlockRows;
-        const long long row = slot[i] * p.head_k + r % (uint32_t)p.head_k;
+        const long long row = slot[i] * p.head_k + (r - token[i] * (uint32_t)p.head_k);
         scale[i] = scales[row];
 #pragma unroll
         for (int c = 0; c < C::kChunks; ++c) {
@@ -195,8 +245,7 @@ __global__ void __launch_bounds__(kThreads) da_kv_read_kernel(const KvRowsParams
     for (int i = 0; i < kRows; ++i) {
         const uint32_t r = first + i * kBlockRows;
         if (r >= total) continue;
-        const uint32_t token = r / (uint32_t)p.head_k, head = r - token * (uint32_t)p.head_k;
-        T *row = dst + (long long)token * dst_stride + (long long)head * D;
+        T *row = dst + (long long)token[i] * dst_stride + (long long)(r - token[i] * (uint32_t)p.head_k) * D;
 #pragma unroll
         for (int c = 0; c < C::kChunks; ++c) {
             float x[8];
@@ -215,20 +264,16 @@ cudaError_t launch_rows(const KvRowsParams &p, bool write, cudaStream_t s) {
     const bool many = p.rows > 4u * kBlockRows * 148u;
     const uint32_t per_block = kBlockRows * (many ? 4u : 1u);
     const dim3 grid((p.rows + per_block - 1) / per_block, 2);
+    count_launch();
     if (write) {
         if constexpr (!std::is_same<T, float>::value) {
-            if (many) da_kv_write_kernel<T, D, KVQ, 4><<<grid, kThreads, 0, s>>>(p);
-            else da_kv_write_kernel<T, D, KVQ, 1><<<grid, kThreads, 0, s>>>(p);
-        } else {
-            return cudaErrorInvalidValue;
+            return many ? launch_kernel(da_kv_write_kernel<T, D, KVQ, 4>, grid, kThreads, 0, s, true, p)
+                        : launch_kernel(da_kv_write_kernel<T, D, KVQ, 1>, grid, kThreads, 0, s, true, p);
         }
-    } else if (many) {
-        da_kv_read_kernel<T, D, KVQ, 4><<<grid, kThreads, 0, s>>>(p);
-    } else {
-        da_kv_read_kernel<T, D, KVQ, 1><<<grid, kThreads, 0, s>>>(p);
+        return cudaErrorInvalidValue;
     }
-    count_launch();
-    return cudaGetLastError();
+    return many ? launch_kernel(da_kv_read_kernel<T, D, KVQ, 4>, grid, kThreads, 0, s, true, p)
+                : launch_kernel(da_kv_read_kernel<T, D, KVQ, 1>, grid, kThreads, 0, s, true, p);
 }
 
 template <typename T, int D>

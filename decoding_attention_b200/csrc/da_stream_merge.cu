@@ -41,10 +41,10 @@ struct RowSum {
 
 // kWarps warps share a row; with kWarps = 1 a warp does `heads_per_warp` rows of a sequence one after another.
 template <int D, int kWarps>
-__global__ void __launch_bounds__(kMergeWarps * 32) da_stream_merge_kernel(const StreamMergeParams p, const int heads_per_warp) {
+__global__ void __launch_bounds__(kMergeWarps * 32, kWarps == 1 ? 5 : 3) da_stream_merge_kernel(const StreamMergeParams p, const int heads_per_warp) {
     constexpr int kVec = RowSum<D>::kVec;
     constexpr int kRows = kMergeWarps / kWarps;
-    constexpr int kBatch = D <= 128 ? 8 : 4;  // records in flight
+    constexpr int kBatch = (kWarps == 1 ? 4 : 8) / kVec;  // records in flight: fewer where rows are many, for more warps
     __shared__ float4 acc_s[kWarps > 1 ? kMergeWarps : 1][kVec * 32];
     __shared__ float2 stat_s[kWarps > 1 ? kMergeWarps : 1];  // reference maximum and sum of each warp
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
@@ -197,16 +197,15 @@ cudaError_t launch_merge_warps(const StreamMergeParams &p, int heads_per_warp, c
 template <int D>
 cudaError_t launch_merge_dim(const StreamMergeParams &p, cudaStream_t s, bool overlap) {
     // Parts of a row, as far as the host can tell: those of the prefix and the sequence's share of the spans.  A warp for
-    // every four of them, if the blocks then still fit the SMs at once (three each): a second wave costs as much as the
-    // first, a warp that finds nothing to do too.  More blocks than that with a warp a row: several rows a warp.
+    // every four of them, if the blocks then still fit the SMs at once (three each).  Otherwise a warp a row, and above 740 blocks (five an SM) two
+    // rows a warp, which share the search for their parts.
     const int parts = (p.prefix_o ? p.prefix.max_parts : 0) + 1 + p.s.spans / p.s.batch;
-    auto fits = [&](int warps) { return (long long)p.s.batch * ((p.s.head_q * warps + 7) / 8) <= 444; };
-    if (parts > 16 && fits(8)) return launch_merge_warps<D, 8>(p, 1, s, overlap);
-    if (parts > 8 && fits(4)) return launch_merge_warps<D, 4>(p, 1, s, overlap);
-    if (parts > 4 && fits(2)) return launch_merge_warps<D, 2>(p, 1, s, overlap);
-    int heads = 1;
-    while (heads < 8 && (long long)p.s.batch * ((p.s.head_q + 8 * heads - 1) / (8 * heads)) > 444 && 8 * heads < p.s.head_q) heads *= 2;
-    return launch_merge_warps<D, 1>(p, heads, s, overlap);
+    auto blocks = [&](int warps) { return (long long)p.s.batch * ((p.s.head_q * warps + 7) / 8); };
+    if (parts > 16 && blocks(8) <= 444) return launch_merge_warps<D, 8>(p, 1, s, overlap);
+    if (parts > 8 && blocks(4) <= 444) return launch_merge_warps<D, 4>(p, 1, s, overlap);
+    if (parts > 4 && blocks(2) <= (parts > 8 ? 888 : 444)) return launch_merge_warps<D, 2>(p, 1, s, overlap);
+    const bool many = blocks(1) > 740 && p.s.head_q > 8;
+    return launch_merge_warps<D, 1>(p, many ? 2 : 1, s, overlap);
 }
 
 }  // namespace
