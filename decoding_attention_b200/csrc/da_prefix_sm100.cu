@@ -244,8 +244,8 @@ da_prefix_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap tm_q,
                 for (int ks = 0; ks < kKeys / 16; ++ks)
                     umma_ts(tmem + C::kColO + l * D, tmem + C::kColP + l * C::kStrideP + ks * 8,
                             vd + (uint64_t)((ks * 16 * 128) >> 4), kIdescPV, (j >= 2 || ks > 0) ? 1u : 0u, leader);
-                umma_commit(&pv_done[l], leader);
                 if (x.split || l == 1) umma_commit(&slot_empty[st], leader);
+                umma_commit(&pv_done[l], leader);  // (last: what the threads wait for before the block ends)
                 if (j + 2 < steps) scores(j + 2);
             }
             base += tiles;
