@@ -56,7 +56,59 @@ cudaError_t launch_stream(int dim, int kind, bool bf16, const StreamParams &p, c
     }
 }
 
+namespace {
+// Whether the tensor-core kernel for codes takes the call: 8-bit codes of head dims and groups that it has, in pages that a
+// TMA box can fetch, and pieces that are worth its 128-key tiles.  With no more (sequence, KV head) pairs than CTA slots it
+// is the faster one at any length (one sequence of 1 500 keys, 8 KV heads: 8.7 us against 10.5); with more, a CTA works
+// through several short sequences, and a piece costs it more (1 000 sequences of 65-130 keys: 96 against 74 us; 256 of
+// 1 000-2 000: 150 against 175 us).  The lengths are on the device: what the cache holds a sequence is what there is to go by.
+bool on_codes_kernel(int dim, int kind, const StreamParams &p, int sms) {
+    if ((kind != DA_KV_FP8_E4M3 && kind != DA_KV_INT8) || (dim != 96 && dim != 128) || p.group > codes_heads() || p.rows == 0) return false;
+    if (p.block_table && p.page_shift < 4) return false;
+    if ((int64_t)p.batch * p.head_k <= (int64_t)sms * codes_ctas()) return true;
+    int64_t keys = p.rows / p.batch;
+    if (p.block_table && ((int64_t)p.table_blocks << p.page_shift) < keys) keys = (int64_t)p.table_blocks << p.page_shift;
+    return keys >= 512;
+}
+// Codes of a cache as [rows][head_k][dim] bytes.
+int codes_map(const void *base, const StreamParams &p, int dim, CUtensorMap *out) {
+    const uint64_t dims[3] = {(uint64_t)dim, (uint64_t)p.head_k, (uint64_t)p.rows};
+    const uint64_t strides[2] = {(uint64_t)dim, (uint64_t)dim * p.head_k};
+    const uint32_t box[3] = {128, 1, p.block_table && p.page_shift < 7 ? 1u << p.page_shift : 128u};
+    return encode_tensor_map(base, 3, dims, strides, box, true, 2, out);
+}
+}  // namespace
+
+// Launches the kernel that plan_stream chose; a DA_* status.
+int run_stream(int dim, int kind, bool bf16, const StreamParams &p, cudaStream_t s) {
+    cudaError_t e;
+    if (p.on_codes) {
+        int *status = nullptr;
+        CUtensorMap tm_k, tm_v;
+        int rc = xmerge_status_ptr(&status);
+        if (rc == DA_OK) rc = codes_map(p.k, p, dim, &tm_k);
+        if (rc == DA_OK) rc = codes_map(p.v, p, dim, &tm_v);
+        if (rc != DA_OK) return rc;
+        e = launch_codes(dim, kind, p, status, tm_k, tm_v, s);
+    } else {
+        e = launch_stream(dim, kind, bf16, p, s, true);
+    }
+    if (e != cudaSuccess) return failf(DA_ERR_CUDA, "decode kernel launch: %s", cudaGetErrorString(e));
+    return DA_OK;
+}
+
 void plan_stream(int dim, int kind, int sms, StreamParams *p) {
+    p->on_codes = on_codes_kernel(dim, kind, *p, sms) ? 1 : 0;
+    if (p->on_codes) {
+        const int slots = sms * codes_ctas();
+        p->chunks = 1;
+        p->spans = slots > p->head_k ? slots / p->head_k : 1;
+        p->snap = 128;
+        p->piece_cost = 128;  // a piece's start and end take about as long as a tile
+        p->min_span = 256;
+        return;
+    }
+    p->snap = 32;
     const StreamShape shape = stream_shape(dim, kind, p->group);
     p->chunks = (p->group + shape.heads - 1) / shape.heads;
     const int streams = p->head_k * p->chunks;
@@ -350,8 +402,9 @@ int da_quant_decode_fwd(const da_quant_decode_args_t *a) {
     m.o = a->o;
     m.lse = a->lse;
     cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
-    cudaError_t e = launch_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream, true);
-    if (e == cudaSuccess) e = launch_stream_merge(m, stream, true);
+    rc = run_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream);
+    if (rc != DA_OK) return rc;
+    const cudaError_t e = launch_stream_merge(m, stream);
     if (e != cudaSuccess) return failf(DA_ERR_CUDA, "decode kernel launch: %s", cudaGetErrorString(e));
     return DA_OK;
 }
@@ -424,8 +477,10 @@ int da_prefix_decode_fwd(const da_prefix_decode_args_t *a) {
         m.s.own_lse = m.s.own_o + rows * a->dim;
         m.s.chained = 1;
     }
-    if (e == cudaSuccess) e = launch_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream, true);
-    if (e == cudaSuccess) e = launch_stream_merge(m, stream, true);
+    if (e != cudaSuccess) return failf(DA_ERR_CUDA, "shared-prefix kernel launch: %s", cudaGetErrorString(e));
+    rc = run_stream(m.dim, a->kv_dtype, a->is_bf16 != 0, m.s, stream);
+    if (rc != DA_OK) return rc;
+    e = launch_stream_merge(m, stream);
     if (e != cudaSuccess) return failf(DA_ERR_CUDA, "shared-prefix kernel launch: %s", cudaGetErrorString(e));
     return DA_OK;
 }

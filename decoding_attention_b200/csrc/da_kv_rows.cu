@@ -109,7 +109,6 @@ __global__ void __launch_bounds__(kThreads) da_kv_write_kernel(const KvRowsParam
     uint8_t *__restrict__ cache = static_cast<uint8_t *>(blockIdx.y ? p.v_cache : p.k_cache);
     float *__restrict__ scales = blockIdx.y ? p.v_scale : p.k_scale;
     pdl_wait();  // the kernel before this one may still be running
-    pdl_launch_dependents();
     const int lane = threadIdx.x % L;
     const uint32_t first = blockIdx.x * (uint32_t)(kBlockRows * kRows) + threadIdx.x / L;
 
@@ -184,6 +183,7 @@ __global__ void __launch_bounds__(kThreads) da_kv_write_kernel(const KvRowsParam
             store_codes<KVQ>(cache + dst[i] * kRowBytes + (lane + c * L) * (KVQ == 3 ? 4 : 8), x, odd ? 0.0f : f);
         }
     }
+    pdl_launch_dependents();  // (at the end: see da_stream_merge.cu)
 }
 
 template <typename T>
@@ -210,7 +210,6 @@ __global__ void __launch_bounds__(kThreads) da_kv_read_kernel(const KvRowsParams
     const uint8_t *__restrict__ cache = static_cast<const uint8_t *>(blockIdx.y ? p.v_cache : p.k_cache);
     const float *__restrict__ scales = blockIdx.y ? p.v_scale : p.k_scale;
     pdl_wait();
-    pdl_launch_dependents();
     const int lane = threadIdx.x % C::kLanes;
     const uint32_t total = p.rows;
     const uint32_t first = blockIdx.x * (uint32_t)(kBlockRows * kRows) + threadIdx.x / C::kLanes;
@@ -255,6 +254,7 @@ __global__ void __launch_bounds__(kThreads) da_kv_read_kernel(const KvRowsParams
             store8<T>(row + (lane + c * C::kLanes) * 8, x);
         }
     }
+    pdl_launch_dependents();
 }
 
 // Rows of a thread.  Few rows: one each, to spread them over the SMs.

@@ -11,8 +11,8 @@ namespace da {
 
 // The batch's work is an axis on which sequence b takes piece_cost + len(b) units: what a piece costs however short it is,
 // in keys, then its keys.  The axis is cut into `spans` equal spans, one per CTA (and head block); a cut falls on a multiple
-// of kSpanKeys keys of its sequence.
-constexpr int kSpanKeys = 32;
+// of `snap` keys of its sequence.
+constexpr int kSpanUnits = 32;  // spans are multiples of this
 
 struct StreamParams {
     const void *q;                 // [batch, head_q, dim]
@@ -33,12 +33,13 @@ struct StreamParams {
     int chunks;                    // warps that share a KV head (each has up to 8 NT of its query heads)
     int head_warps, key_warps;     // a CTA's eight warps: so many (KV head, chunk) streams x so many parts of the keys
     int spans, min_span;           // CTAs along the axis; no span is shorter than min_span units
-    int piece_cost;
+    int piece_cost, snap;
     int is_alibi, q_bf16;
     float scale_log2;              // softmax scale * log2(e)
     // Launched while the prefix kernel still runs: the grid then ends only after that one has, so that whoever waits for
     // this grid may read the other's results too.
     int chained;
+    int on_codes;                  // host side: the kernel that takes the call (plan_stream)
 };
 
 // kind: 0 the type of q, 1 FP8 e4m3, 2 int8, 3 int4.
@@ -55,6 +56,14 @@ cudaError_t launch_stream_d96(int kind, bool bf16, const StreamParams &p, cudaSt
 cudaError_t launch_stream_d128(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
 cudaError_t launch_stream_d256(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
 
+// The tensor-core kernel for 8-bit codes (da_codes_sm100.cu), head dims 96 and 128, groups of at most codes_heads() query
+// heads: p.spans spans, cuts at multiples of 128 keys, pages of 16 keys or more.  kind: 1 FP8 e4m3, 2 int8.  tm_k, tm_v:
+// [rows][head_k][dim] bytes, box {128, 1, 128 keys or a shorter page} with the 128-byte swizzle; rows beyond p.rows come as zeros.
+int codes_heads();
+int codes_ctas();  // per SM
+cudaError_t launch_codes(int dim, int kind, const StreamParams &p, int *status, const CUtensorMap &tm_k, const CUtensorMap &tm_v,
+                         cudaStream_t s);
+
 // o = softmax-weighted sum of a row's pieces: those of the key stream and, with a shared prefix, its parts.
 struct StreamMergeParams {
     StreamParams s;
@@ -64,14 +73,14 @@ struct StreamMergeParams {
     void *o;      // [batch, head_q, dim], rows s.o_row_stride apart
     float *lse;   // optional [batch, head_q]
 };
-cudaError_t launch_stream_merge(const StreamMergeParams &p, cudaStream_t s, bool overlap);
+cudaError_t launch_stream_merge(const StreamMergeParams &p, cudaStream_t s);
 
 // The cut of the axis into spans, the same in the stream kernel and in the merge.
 struct SpanPlan {
     long long units;  // of a span
     long long total;  // of the batch
     int first;        // cu_seq_k[0]
-    int cost;
+    int cost, snap;
 };
 #ifdef __CUDACC__
 // a / b of positions on the axis, which nearly always fit 32 bits (a 64-bit division takes ten times as long).
@@ -82,11 +91,12 @@ __device__ __forceinline__ SpanPlan span_plan(const StreamParams &p) {
     SpanPlan s;
     s.first = p.cu_seq_k[0];
     s.cost = p.piece_cost;
+    s.snap = p.snap;  // a power of two
     const long long keys = (long long)p.cu_seq_k[p.batch] - s.first;
     s.total = (keys > 0 ? keys : 0) + (long long)p.batch * s.cost;
     long long units = axis_div(s.total + p.spans - 1, p.spans);
     if (units < p.min_span) units = p.min_span;
-    s.units = (units + kSpanKeys - 1) / kSpanKeys * kSpanKeys;
+    s.units = (units + kSpanUnits - 1) / kSpanUnits * kSpanUnits;
     return s;
 }
 // Where sequence b, whose keys start at cu, begins on the axis.
@@ -96,8 +106,8 @@ __device__ __forceinline__ long long axis_start(const SpanPlan &s, int b, int cu
 // Keys [begin, end) that span i has of a sequence of `len` keys that begins at `start` on the axis.
 __device__ __forceinline__ void span_piece(const SpanPlan &s, long long i, long long start, int len, int &begin, int &end) {
     const long long lo = i * s.units - start - s.cost, hi = lo + s.units;
-    begin = lo <= 0 ? 0 : (lo >= len ? len : (int)lo / kSpanKeys * kSpanKeys);
-    end = hi <= 0 ? 0 : (hi >= len ? len : (int)hi / kSpanKeys * kSpanKeys);
+    begin = lo <= 0 ? 0 : (lo >= len ? len : (int)lo & -s.snap);
+    end = hi <= 0 ? 0 : (hi >= len ? len : (int)hi & -s.snap);
 }
 #endif
 

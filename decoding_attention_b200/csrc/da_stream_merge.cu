@@ -50,7 +50,6 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kWarps == 1 ? 5 : 3) da_stre
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const int slice = warp % kWarps;  // this warp's parts: slice, slice + kWarps, ...
     const int b = blockIdx.y;
-    pdl_launch_dependents();
     // Where the parts are depends on the lengths alone, which were there before the stream kernel started.
     const SpanPlan plan = span_plan(p.s);
     const int cu = p.s.cu_seq_k[b];
@@ -65,6 +64,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kWarps == 1 ? 5 : 3) da_stre
     if (len > 0) {
         first_span = axis_div(start, plan.units);
         spans = (int)(axis_div(start + plan.cost + len - 1, plan.units) - first_span) + 1;
+        // (lengths that are not cumulative would point outside the workspace)
+        if (first_span < 0 || first_span >= p.s.spans) first_span = spans = 0;
+        if (first_span + spans > p.s.spans) spans = (int)(p.s.spans - first_span);
         int begin, end;
         for (int i = 0; i < 2 && i < spans; ++i) {
             span_piece(plan, first_span + i, start, len, begin, end);
@@ -186,37 +188,41 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kWarps == 1 ? 5 : 3) da_stre
         }
         if (lane == 0 && p.lse) p.lse[row] = x.sum > 0.0f ? x.ref + logf(x.sum) : (x.sum == 0.0f ? -INFINITY : x.sum);
     }
+    // The next call's kernel may start now, and not earlier: its big blocks, put down between the small ones of this kernel,
+    // would find the register file in pieces, and some SMs then hold one block less until their first ones end (256
+    // sequences of 512-4096 FP8 keys, calls back to back: 265 us where 212 are enough).
+    pdl_launch_dependents();
 }
 
 template <int D, int kWarps>
-cudaError_t launch_merge_warps(const StreamMergeParams &p, int heads_per_warp, cudaStream_t s, bool overlap) {
+cudaError_t launch_merge_warps(const StreamMergeParams &p, int heads_per_warp, cudaStream_t s) {
     const int heads = kMergeWarps / kWarps * heads_per_warp;
     return launch_kernel(da_stream_merge_kernel<D, kWarps>, dim3((p.s.head_q + heads - 1) / heads, p.s.batch), kMergeWarps * 32, 0, s,
-                         overlap, p, heads_per_warp);
+                         true, p, heads_per_warp);
 }
 template <int D>
-cudaError_t launch_merge_dim(const StreamMergeParams &p, cudaStream_t s, bool overlap) {
+cudaError_t launch_merge_dim(const StreamMergeParams &p, cudaStream_t s) {
     // Parts of a row, as far as the host can tell: those of the prefix and the sequence's share of the spans.  A warp for
-    // every four of them, if the blocks then still fit the SMs at once (three each).  Otherwise a warp a row, and above 740 blocks (five an SM) two
-    // rows a warp, which share the search for their parts.
+    // every four of them, if the blocks then still fit the SMs at once (three each).  Otherwise a warp a row, and above 740
+    // blocks (five an SM) two rows a warp, which share the search for their parts.
     const int parts = (p.prefix_o ? p.prefix.max_parts : 0) + 1 + p.s.spans / p.s.batch;
     auto blocks = [&](int warps) { return (long long)p.s.batch * ((p.s.head_q * warps + 7) / 8); };
-    if (parts > 16 && blocks(8) <= 444) return launch_merge_warps<D, 8>(p, 1, s, overlap);
-    if (parts > 8 && blocks(4) <= 444) return launch_merge_warps<D, 4>(p, 1, s, overlap);
-    if (parts > 4 && blocks(2) <= (parts > 8 ? 888 : 444)) return launch_merge_warps<D, 2>(p, 1, s, overlap);
+    if (parts > 16 && blocks(8) <= 444) return launch_merge_warps<D, 8>(p, 1, s);
+    if (parts > 8 && blocks(4) <= 444) return launch_merge_warps<D, 4>(p, 1, s);
+    if (parts > 4 && blocks(2) <= (parts > 8 ? 888 : 444)) return launch_merge_warps<D, 2>(p, 1, s);
     const bool many = blocks(1) > 740 && p.s.head_q > 8;
-    return launch_merge_warps<D, 1>(p, many ? 2 : 1, s, overlap);
+    return launch_merge_warps<D, 1>(p, many ? 2 : 1, s);
 }
 
 }  // namespace
 
-cudaError_t launch_stream_merge(const StreamMergeParams &p, cudaStream_t s, bool overlap) {
+cudaError_t launch_stream_merge(const StreamMergeParams &p, cudaStream_t s) {
     count_launch();
     switch (p.dim) {
-        case 64: return launch_merge_dim<64>(p, s, overlap);
-        case 96: return launch_merge_dim<96>(p, s, overlap);
-        case 128: return launch_merge_dim<128>(p, s, overlap);
-        case 256: return launch_merge_dim<256>(p, s, overlap);
+        case 64: return launch_merge_dim<64>(p, s);
+        case 96: return launch_merge_dim<96>(p, s);
+        case 128: return launch_merge_dim<128>(p, s);
+        case 256: return launch_merge_dim<256>(p, s);
         default: return cudaErrorInvalidValue;
     }
 }

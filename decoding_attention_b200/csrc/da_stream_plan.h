@@ -14,6 +14,7 @@ bool quantised_kind(int32_t kv_dtype);
 // Fills chunks, head_warps, key_warps, spans and min_span from head_k and group.
 void plan_stream(int dim, int kind, int sms, StreamParams *p);
 size_t stream_piece_bytes(const StreamParams &p, int dim);  // of part_o and part_lse together
+int run_stream(int dim, int kind, bool bf16, const StreamParams &p, cudaStream_t s);
 cudaError_t launch_stream(int dim, int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
 
 }  // namespace da

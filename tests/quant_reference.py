@@ -68,10 +68,11 @@ def attend(q, ks, vs, alibi=False, softmax_scale=None):
 
 def bounds(o, lse, spread, scores, top, n, weight_bits, out_dtype):
     """Tolerances of o and lse.  Softmax weights rounded to `weight_bits` bits: half a step, 2^-weight_bits relative, or
-    2^-25 of the largest weight where fp16 runs into its subnormals (n of them at worst).  Scores: a chain of fp32
+    2^-25 of the largest weight where fp16 runs into its subnormals, 2^-23 of it where weights are fixed-point numbers of
+    22 bits behind the largest one (n of them at worst; the largest weight times its largest code is at most `top`).  Scores: a chain of fp32
     accumulations, 2^-19 of the sum of magnitudes, which moves every weight and the sum alike; exp2 and the
     sums: 2^-19.  Output: half a step of its type."""
     drift = 2.0 ** -19 * (1.0 + scores)
-    tol_o = spread * (2.0 ** -weight_bits + 2 * drift[:, None]) + n * 2.0 ** -25 * top
+    tol_o = spread * (2.0 ** -weight_bits + 2 * drift[:, None]) + n * 2.0 ** -23 * top
     tol_o = tol_o + (o.abs() + tol_o) * torch.finfo(out_dtype).eps / 2 + 2.0 ** -25
     return tol_o, drift + 2.0 ** -21 * torch.nan_to_num(lse.abs(), posinf=0.0)

@@ -301,6 +301,41 @@ def test_decode_queries_of_extreme_size(api):
     check(api, pr, what="q sizes")
 
 
+@pytest.mark.parametrize("dim", [96, 128])
+@pytest.mark.parametrize("kind", KINDS)
+def test_decode_many_short_sequences_of_every_head_layout(api, kind, dim):
+    """More (sequence, KV head) pairs than the GPU holds blocks, a few keys each."""
+    lens = [(i * 53) % 97 for i in range(150)]
+    for hq, hk, page in ((32, 8, 0), (8, 8, 16), (12, 4, 1)):
+        check(api, problem(kind, torch.bfloat16, lens, hq, hk, dim, 26, page=page), alibi=page == 1, what=f"{kind} {hq}/{hk} page {page}")
+
+
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+def test_calls_right_behind_the_writes_of_their_inputs(api, kind):
+    """Fresh caches, memory traffic just before the call (late tiles), long and short sequences in one block."""
+    for seed in range(12):
+        pr = problem(kind, torch.bfloat16, [5000, 20000, 1, 0, 7, 9000], 32, 8, 128, 200 + seed, poison=seed % 2 == 0)
+        junk = torch.full((48 << 20,), float(seed), device=DEV)
+        del junk
+        check(api, pr, what=f"seed {seed}")
+
+
+def test_more_keys_in_a_block_than_its_integers_hold(api):
+    """Equal scores and the largest codes: every weight counts, sums pass 2^31 unless they are taken over in time."""
+    n, hk = 101000, 128
+    g = torch.Generator(device=DEV).manual_seed(27)
+    kc = torch.zeros(n, hk, 128, dtype=torch.int8, device=DEV)
+    vc = torch.full((n, hk, 128), 127, dtype=torch.int8, device=DEV)
+    vc[:, 1::2] = -127
+    ks, vs = torch.ones(n, hk, device=DEV), torch.full((n, hk), 0.5, device=DEV)
+    q = torch.randn(1, hk, 128, device=DEV, generator=g).to(torch.bfloat16)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    o, lse = api.quantized_fwd(q, kc, vc, ks, vs, cu, return_lse=True)
+    want = torch.full((hk, 1), 63.5, device=DEV)
+    want[1::2] = -63.5
+    assert (o[0].float() == want).all() and (lse - math.log(n)).abs().max() <= 2e-5
+
+
 def test_nan_and_infinity_reach_the_sequences_that_hold_them_only(api):
     pr = problem("int8", torch.bfloat16, [100, 333, 50], 8, 2, 128, 22, poison=False)
     pr["vs"][100 + 200, 1] = math.nan
