@@ -121,8 +121,8 @@ struct SpanWalk {
             start = p.cu_seq_k[b];
             const long long at = axis_start(s, b, start);
             if (at >= (span + 1) * s.units) return false;
-            len = p.cu_seq_k[b + 1] - start;
-            if (len <= 0) continue;
+            len = sequence_keys(p, b, start);
+            if (len == 0) continue;
             span_piece(s, span, at, len, begin, end);
             if (begin < end) return true;
         }

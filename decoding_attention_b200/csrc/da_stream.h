@@ -1,6 +1,8 @@
 // Launch parameters of the key-stream decode kernels (da_stream_kernel.cuh) and of the merge behind them.
 #pragma once
 
+#include <climits>
+
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -33,7 +35,7 @@ struct StreamParams {
     int chunks;                    // warps that share a KV head (each has up to 8 NT of its query heads)
     int head_warps, key_warps;     // a CTA's eight warps: so many (KV head, chunk) streams x so many parts of the keys
     int spans, min_span;           // CTAs along the axis; no span is shorter than min_span units
-    int piece_cost, snap;
+    int piece_cost, snap;          // piece_cost + snap <= min_span: a sequence has keys in its first or second span
     int is_alibi, q_bf16;
     float scale_log2;              // softmax scale * log2(e)
     // Launched while the prefix kernel still runs: the grid then ends only after that one has, so that whoever waits for
@@ -98,6 +100,12 @@ __device__ __forceinline__ SpanPlan span_plan(const StreamParams &p) {
     if (units < p.min_span) units = p.min_span;
     s.units = (units + kSpanUnits - 1) / kSpanUnits * kSpanUnits;
     return s;
+}
+// Keys of sequence b, which starts at cu.  (The bound keeps the indices of a tile behind the last key inside 32 bits; a
+// cache has fewer rows.)
+__device__ __forceinline__ int sequence_keys(const StreamParams &p, int b, int cu) {
+    const long long n = (long long)p.cu_seq_k[b + 1] - cu;
+    return n < 0 ? 0 : (n > INT_MAX - 1024 ? INT_MAX - 1024 : (int)n);
 }
 // Where sequence b, whose keys start at cu, begins on the axis.
 __device__ __forceinline__ long long axis_start(const SpanPlan &s, int b, int cu) {

@@ -47,6 +47,7 @@ struct StreamCfg {
     static constexpr int KW = RB / 16;                     // words of a K row in a lane (a quarter of the row)
     static constexpr int VW = (RB + 31) / 32;              // words of a V row in a lane (an eighth; the last may be half)
     static constexpr int CPR = RB / 16;                    // 16-byte chunks of a row
+    static_assert(TK * CPR % 32 == 0, "all lanes take part in every copy of a tile");
     static constexpr int kScaleBytes = kQuant ? TK * 8 : 0;
     static constexpr int kStageBytes = 2 * TK * RB + kScaleBytes;
     static constexpr bool kTwoCtas = D <= 128 && NT == 1 && RB <= 128;
@@ -248,8 +249,8 @@ struct PieceCursor {
             start = p.cu_seq_k[b];
             const long long at = axis_start(s, b, start);
             if (at >= (span + 1) * s.units) return false;
-            len = p.cu_seq_k[b + 1] - start;
-            if (len <= 0) continue;
+            len = sequence_keys(p, b, start);
+            if (len == 0) continue;
             span_piece(s, span, at, len, begin, end);
             if (begin < end) return true;
         }

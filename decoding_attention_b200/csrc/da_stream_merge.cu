@@ -54,8 +54,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kWarps == 1 ? 5 : 3) da_stre
     const SpanPlan plan = span_plan(p.s);
     const int cu = p.s.cu_seq_k[b];
     const long long start = axis_start(plan, b, cu);
-    int len = p.s.cu_seq_k[b + 1] - cu;
-    if (len < 0) len = 0;
+    const int len = sequence_keys(p.s, b, cu);
 
     // stream parts: spans first_span .. first_span + spans - 1, or the whole sequence in own_o
     long long first_span = 0;

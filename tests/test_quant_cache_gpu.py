@@ -310,6 +310,26 @@ def test_decode_many_short_sequences_of_every_head_layout(api, kind, dim):
         check(api, problem(kind, torch.bfloat16, lens, hq, hk, dim, 26, page=page), alibi=page == 1, what=f"{kind} {hq}/{hk} page {page}")
 
 
+@pytest.mark.parametrize("page", [16, 64, 512])
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+def test_decode_long_ragged_pages_with_bias(api, kind, page):
+    """Tiles of several pages, pages of several tiles, cuts and ends inside both, walked from the end."""
+    for lens, hq, hk, dim in (([6001, 0, 129, 12345, 128, 2], 8, 4, 96), ([40001], 16, 4, 128), ([3000] * 5 + [1], 5, 5, 128)):
+        check(api, problem(kind, torch.float16, lens, hq, hk, dim, 28, page=page), alibi=True, what=f"{lens} {hq}/{hk}")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_lengths_that_are_not_cumulative_stay_inside(api, kind):
+    """What comes out is unspecified then; nothing around the output changes and the next call is right."""
+    pr = problem(kind, torch.bfloat16, [700, 20, 300, 5, 60], 32, 8, 128, 29)
+    for cu in ([0, 900, 100, 2000, 50, 1085], [500, 400, 300, 200, 100, 0], [-7, 3, 2 ** 31 - 1, 0, 5, 9], [2 ** 31 - 1] * 5 + [-2 ** 31]):
+        wide = torch.full((5, 40, 128), 3.0, dtype=torch.bfloat16, device=DEV)
+        api.quantized_fwd(pr["q"], pr["kc"], pr["vc"], pr["ks"], pr["vs"], torch.tensor(cu, dtype=torch.int32, device=DEV),
+                          out=wide[:, 4:36])
+        assert (wide[:, :4] == 3.0).all() and (wide[:, 36:] == 3.0).all()
+    check(api, pr)
+
+
 @pytest.mark.parametrize("kind", ["fp8", "int8"])
 def test_calls_right_behind_the_writes_of_their_inputs(api, kind):
     """Fresh caches, memory traffic just before the call (late tiles), long and short sequences in one block."""
