@@ -304,12 +304,26 @@ PrefixGrid plan_prefix(int sms, int batch, int head_k, int group, int prefix_len
     g.pairs = (g.row_tiles + 1) / 2;
     g.key_tiles = (prefix_len + 127) / 128;
     const int64_t total = (int64_t)head_k * g.pairs * g.key_tiles;
+    g.total = (int)total;
+    g.sms = sms;
     g.cta_tiles = (int)((total + sms - 1) / sms);
     g.ctas = (int)((total + g.cta_tiles - 1) / g.cta_tiles);
     // parts of a unit: the runs that touch it, twice where its streams share one row tile
     const int runs = (g.key_tiles + g.cta_tiles - 2) / g.cta_tiles + 1;
     g.max_parts = runs * (g.row_tiles % 2 ? 2 : 1);
     return g;
+}
+
+// What a key of the sequences' own costs an SM, in 1/65536 of a key tile of the prefix; 0 where the prefix does not fill the
+// SMs anyway.  Measured: a key tile of two row tiles takes an SM 2.6 us at dim 128, an SM alone streams 54 GB/s of 16-bit
+// rows, and no format goes below 7 ns for a key and KV head of 128 columns and eight query heads.
+int own_cost(const StreamParams &s, const PrefixGrid &g, int dim, int kind) {
+    if (g.total < 2 * g.sms) return 0;
+    const double tile = (dim <= 64 ? 1800.0 : 2600.0) * g.row_tiles / (2 * g.pairs);
+    const double bytes = kind == DA_KV_SAME_AS_Q ? 4.0 * dim : (kind == DA_KV_INT4 ? 1.0 : 2.0) * dim + 8;
+    const double memory = bytes / 54.0, work = 7.0 * ((s.group + 7) / 8) * dim / 128;
+    const double share = s.head_k * (memory > work ? memory : work) / tile * 65536.0;
+    return share < 1.0 ? 1 : (share > 1e9 ? 1000000000 : (int)share);
 }
 
 struct PrefixPlan {
@@ -352,6 +366,8 @@ PrefixPlan fill_prefix(const da_prefix_decode_args_t *a, int sms, StreamParams *
     memset(&plan, 0, sizeof(plan));
     if (a->prefix_len > 0) {
         plan.grid = plan_prefix(sms, s->batch, s->head_k, s->group, (int)a->prefix_len);
+        plan.grid.own_cost = own_cost(*s, plan.grid, (int)a->dim, a->kv_dtype);
+        if (plan.grid.own_cost) s->beside = plan.grid;
         plan.parts = ((size_t)plan.grid.max_parts * rows * row + 3) / 4 * 4;
         plan.own = (rows * row + 3) / 4 * 4;
     }

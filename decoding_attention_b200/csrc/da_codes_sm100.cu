@@ -588,7 +588,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
     }
 
     if (!ok && lane == 0) atomicExch(status, kStatusWaitTimeout);
-    if (p.chained) pdl_wait();
+    if (stays_for_prefix(p)) pdl_wait();
     __syncthreads();
     if (warp == 5) {
         tc_fence_after();

@@ -16,10 +16,26 @@ struct PrefixGrid {
     int row_tiles;   // row tiles of a KV head
     int pairs;       // units of a KV head: (row_tiles + 1) / 2
     int key_tiles;   // 128-key tiles of the prefix
-    int cta_tiles;   // of a CTA
+    int cta_tiles;   // of a CTA; at least, if own_cost is set
     int ctas;
     int max_parts;   // most partial results of a row
+    int total;       // key tiles of all units
+    // The tensor cores' work on the prefix and the memory's on the sequences' own keys go side by side, each on its SMs:
+    // the runs become as long as they have to be for both to end together, and the CTAs without a run leave their SMs to
+    // the key stream.  How many own keys there are is known on the device only.
+    int own_cost;    // of an own key, in 1/65536 of a key tile's; 0: no sharing
+    int sms;
 };
+constexpr int kShareTiles = 4;  // the prefix keeps a quarter of the SMs
+
+// Key tiles of a CTA next to so many own keys (the same in all three kernels of a call).
+__host__ __device__ inline int prefix_run(const PrefixGrid &g, long long keys) {
+    const long long prefix = (long long)g.total << 16, own = keys * g.own_cost;
+    if (own < prefix / 8) return g.cta_tiles;  // (not worth the longer runs: 170 us instead of 166 with 9 % of own work)
+    const long long run = (prefix + own) / ((long long)g.sms << 16) + 1;
+    const long long most = ((long long)g.total * kShareTiles + g.sms - 1) / g.sms;
+    return (int)(run > most ? most : (run < g.cta_tiles ? g.cta_tiles : run));
+}
 
 struct PrefixParams {
     PrefixGrid grid;
@@ -30,7 +46,7 @@ struct PrefixParams {
     int page_shift;
     int prefix_len;
     int batch, head_q, head_k, group, dim;
-    const int *cu_seq_k;                     // lengths of the sequences' own keys (ALiBi)
+    const int *cu_seq_k;                     // lengths of the sequences' own keys
     int is_alibi;
     float scale_log2;
     float *part_o, *part_lse;                // [max_parts][batch][head_q][dim], [max_parts][batch][head_q]

@@ -116,8 +116,12 @@ da_prefix_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap tm_q,
     pdl_wait();  // the kernel before this call's may still be running
     pdl_launch_dependents();
 
-    const PrefixGrid g = p.grid;
-    const long long total = (long long)p.head_k * g.pairs * g.key_tiles;
+    PrefixGrid g = p.grid;
+    if (g.own_cost) {
+        const long long keys = (long long)p.cu_seq_k[p.batch] - p.cu_seq_k[0];
+        g.cta_tiles = prefix_run(g, keys > 0 ? keys : 0);
+    }
+    const long long total = g.total;
     const long long begin = (long long)blockIdx.x * g.cta_tiles;
     const long long end = begin + g.cta_tiles < total ? begin + g.cta_tiles : total;
     // With ALiBi the scores grow towards the end of the prefix: walked back to front, the first tiles set the maxima.

@@ -39,8 +39,9 @@ struct StreamParams {
     int is_alibi, q_bf16;
     float scale_log2;              // softmax scale * log2(e)
     // Launched while the prefix kernel still runs: the grid then ends only after that one has, so that whoever waits for
-    // this grid may read the other's results too.
+    // this grid may read the other's results too (stays_for_prefix).
     int chained;
+    PrefixGrid beside;             // the prefix kernel's, if the SMs are shared with it (own_cost)
     int on_codes;                  // host side: the kernel that takes the call (plan_stream)
 };
 
@@ -96,7 +97,15 @@ __device__ __forceinline__ SpanPlan span_plan(const StreamParams &p) {
     s.snap = p.snap;  // a power of two
     const long long keys = (long long)p.cu_seq_k[p.batch] - s.first;
     s.total = (keys > 0 ? keys : 0) + (long long)p.batch * s.cost;
-    long long units = axis_div(s.total + p.spans - 1, p.spans);
+    int spans = p.spans;
+    if (p.beside.own_cost) {
+        // As many spans as the SMs that the prefix leaves free take in whole waves.
+        const int run = prefix_run(p.beside, keys > 0 ? keys : 0);
+        const int left = p.beside.sms - (p.beside.total + run - 1) / run;
+        if (run > p.beside.cta_tiles && left > 0) spans = (int)((long long)spans * (p.beside.sms / left * left) / p.beside.sms);
+        if (spans < 1) spans = 1;
+    }
+    long long units = axis_div(s.total + spans - 1, spans);
     if (units < p.min_span) units = p.min_span;
     s.units = (units + kSpanUnits - 1) / kSpanUnits * kSpanUnits;
     return s;
@@ -106,6 +115,11 @@ __device__ __forceinline__ SpanPlan span_plan(const StreamParams &p) {
 __device__ __forceinline__ int sequence_keys(const StreamParams &p, int b, int cu) {
     const long long n = (long long)p.cu_seq_k[b + 1] - cu;
     return n < 0 ? 0 : (n > INT_MAX - 1024 ? INT_MAX - 1024 : (int)n);
+}
+// Whether this block waits for the prefix kernel before it ends.  One block is enough for the grid's end to come after; where
+// the SMs are shared with the prefix the others make room for those that have not started.
+__device__ __forceinline__ bool stays_for_prefix(const StreamParams &p) {
+    return p.chained && (!p.beside.own_cost || (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1));
 }
 // Where sequence b, whose keys start at cu, begins on the axis.
 __device__ __forceinline__ long long axis_start(const SpanPlan &s, int b, int cu) {

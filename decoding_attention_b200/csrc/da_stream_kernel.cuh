@@ -288,10 +288,11 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
 
     if (!p.chained) pdl_wait();  // the kernel before this call's may still be running
     pdl_launch_dependents();
+    const bool stays = stays_for_prefix(p);
     const SpanPlan plan = span_plan(p);
     const long long span = blockIdx.x;
     if (span * plan.units >= plan.total) {
-        if (p.chained) pdl_wait();
+        if (stays) pdl_wait();
         return;
     }
 
@@ -811,7 +812,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                 }
         }
     }
-    if (p.chained) pdl_wait();
+    if (stays) pdl_wait();
 }
 
 template <int KIND, int D, int NT>

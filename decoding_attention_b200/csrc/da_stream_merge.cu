@@ -76,12 +76,14 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kWarps == 1 ? 5 : 3) da_stre
         pdl_wait();
         return;
     }
+    PrefixGrid grid = p.prefix;
+    if (p.prefix_o) grid.cta_tiles = prefix_run(grid, plan.total - (long long)p.s.batch * plan.cost);
     bool waited = false;
     for (int r = 0; r < (kWarps == 1 ? heads_per_warp : 1); ++r) {
         // (past the last head a row is done twice, alike)
         const int head = min((blockIdx.x * kRows + warp / kWarps) * (kWarps == 1 ? heads_per_warp : 1) + r, p.s.head_q - 1);
         const long long row = (long long)b * p.s.head_q + head;
-        const int prefix_parts = p.prefix_o ? prefix_parts_of(p.prefix, head / p.s.group, b) : 0;
+        const int prefix_parts = p.prefix_o ? prefix_parts_of(grid, head / p.s.group, b) : 0;
         const int parts = prefix_parts + (whole ? 1 : spans);
         // Record of part i: its row and its log-sum-exp; NULL for a span that got none of the sequence's keys.
         auto locate = [&](int i, const float *&o, const float *&lse) {

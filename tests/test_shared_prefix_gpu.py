@@ -164,6 +164,41 @@ def test_long_prefix_many_sequences(api):
     check(api, problem(torch.float16, 3300, lens, 32, 1, 64, 15), alibi=True, what="MQA")
 
 
+# Enough key tiles to fill the GPU: the SMs are divided by the lengths that the device finds.
+@pytest.mark.parametrize("hq,hk,dim,batch", [(32, 8, 128, 70), (16, 16, 64, 130), (24, 3, 96, 150), (64, 1, 128, 90)])
+@pytest.mark.parametrize("kind", [None, "fp8", "int8", "int4"])
+def test_own_keys_next_to_a_long_prefix(api, hq, hk, dim, batch, kind):
+    prefix = 2500 if hk > 1 else 5000
+    for top in (3, 130, 900):  # hardly any own keys, some, more than the prefix
+        lens = [(i * 37) % (top + 1) for i in range(batch)]
+        page = 64 if top == 130 else 0
+        check(api, problem(torch.bfloat16, prefix, lens, hq, hk, dim, 30, kind=kind, page=page), alibi=top == 900, what=f"{kind} {top}")
+
+
+def test_replay_with_other_lengths(api):
+    """A captured call is used with lengths that change which SMs do what."""
+    batch, hq, hk, dim, prefix = 70, 32, 8, 128, 2500
+    pr = problem(torch.bfloat16, prefix, [800] * batch, hq, hk, dim, 31)
+    full = pr["cu"].clone()
+    keys = pr["keys"]
+    buf = torch.zeros_like(pr["q"])
+    call(api, pr)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, lse = call(api, pr, out=buf)
+    for n in (800, 0, 1, 300, 20, 799):
+        pr["cu"].copy_((torch.arange(batch + 1, device=DEV) * n).to(torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        o2, lse2 = call(api, pr)
+        assert torch.equal(buf, o2) and torch.equal(lse, lse2)
+        own = [[torch.cat([x[prefix:] for x in side]) for side in keys]][0]
+        pr["keys"] = [[torch.cat((side[b][:prefix], own[i][b * n:(b + 1) * n])) for b in range(batch)] for i, side in enumerate(keys)]
+        check(api, pr, what=f"{n} own keys")
+    pr["cu"].copy_(full)
+
+
 @pytest.mark.parametrize("alibi", [False, True])
 def test_scores_that_rise_and_fall(api, alibi):
     """Row maxima that move by far more than the lazy reference allows, in either direction, and a long softmax scale."""
