@@ -147,7 +147,7 @@ int check_rows_args(const da_kv_rows_args_t *a, bool write) {
     if (a->tokens > 0 && (!a->k || !a->v)) return failf(DA_ERR_INVALID_ARG, "k and v must not be NULL");
     if (a->cache_rows > 0 && (!a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale))
         return failf(DA_ERR_INVALID_ARG, "k_cache, v_cache, k_scale and v_scale must not be NULL");
-    if (a->head_k > INT32_MAX / 256 || a->tokens * a->head_k > (int64_t)INT32_MAX || a->cache_rows > INT64_MAX / 256 / a->head_k)
+    if (a->head_k > INT32_MAX / 256 || a->tokens > INT32_MAX / a->head_k || a->cache_rows > INT64_MAX / 256 / a->head_k)
         return failf(DA_ERR_INVALID_ARG, "tokens * head_k must be below 2^31");
     if (!a->slots && a->tokens > a->cache_rows)
         return failf(DA_ERR_INVALID_ARG, "%lld tokens without slots do not fit %lld cache rows", (long long)a->tokens, (long long)a->cache_rows);

@@ -3,17 +3,24 @@
 //
 //     s_j = c ks_j (q . kc_j) [+ slope (j - (len - 1))],   o = sum_j softmax(s)_j vs_j vc_j
 //
-// Bound: HBM.  A byte of a quantised cache carries one or two elements, each of which becomes an operand of one
-// multiply-add per query head and has to be converted first: at the HBM rate 23 bytes a clock reach an SM, which is more
-// than its CUDA cores can convert to fp32 and multiply.  So the codes are turned into fp16 PAIRS (exact for all three
+// Bound: HBM for 16-bit rows (0.95 of the copy rate next to a prefix); the issue slots for codes.  A byte of a quantised
+// cache carries one or two elements, each of which becomes an operand of one multiply-add per query head and has to be
+// converted first: at the HBM rate 23 bytes a clock reach an SM, which is more than its CUDA cores can convert to fp32 and
+// multiply.  So the codes are turned into fp16 PAIRS (exact for all three
 // formats: byte and nibble pairs by one logic operation into the mantissa of 1024 and one subtraction, e4m3 by the
 // hardware's pair conversion) straight in the registers in which mma.sync wants them, with the KEYS (and for the second
 // product the DIMS) as the 16 rows of a tile and the query heads as its 8 columns:
 //     S^T[16 keys x 8 heads] = K[16 x D] . Q^T,      O^T[D x 8 heads] += V^T[D x 16] . P^T
 // The products' reduction index may be permuted freely, so a lane loads its elements with 16-byte accesses of
 // untransposed rows, and the transposition of V is two byte permutes per pair of keys.  S^T becomes P^T by one movmatrix
-// per 8 keys.  (tcgen05.mma would read e4m3 codes as they lie, but not int4, nor int8 next to fp16 weights, and V's
-// scales would have to go into weights of 3 bits.)
+// per 8 keys.  16 keys of 128 columns and eight heads take 421 (int4), 447 (e4m3) and 574 (int8) instructions, all told:
+// 4 x 65 536 keys with 64 over 8 heads come to 91 us (int4, HBM time 44), 105 (e4m3, 85) and 124 us (int8, 85).
+//
+// For 8-bit codes and groups of up to four heads da_codes_sm100.cu, where the codes themselves are tensor-core operands, is
+// faster.  Tried for the rest and left out: the codes widened to fp16 in shared memory by warps of their own, once a key, as
+// tcgen05 operands (the chain of widening, scores, weights and the other contraction takes 3 000 cycles a tile with the one
+// CTA an SM that fits: 191 us for the int4 case above); and 32 heads a warp, so that a group of 32 is widened once instead
+// of twice (128 sequences of 2 048 int4 keys, 32 heads over one KV head: 51 us, 42 with two warps of 16 heads).
 //
 // q is brought to fp16 with a power of two per head that makes its largest element 1..2 (exact; undone in the score's
 // factor), whatever its own type.  The weights w_j = p_j vs_j are rounded to fp16 after a second factor per head, kept

