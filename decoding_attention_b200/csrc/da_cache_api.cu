@@ -261,6 +261,9 @@ int check_prefix_args(const da_prefix_decode_args_t *a) {
     if (a->head_q / a->head_k > 128) return failf(DA_ERR_UNSUPPORTED, "more than 128 query heads per KV head");
     if (a->batch > 65535 || a->head_q > 65535) return failf(DA_ERR_INVALID_ARG, "batch and head_q must be <= 65535");
     if (a->prefix_len < 0 || a->prefix_len > (1 << 30)) return failf(DA_ERR_INVALID_ARG, "prefix_len must be in [0, 2^30]");
+    // (rows of a KV head in 256s at most) x (keys in 128s) x KV heads are counted in 32 bits
+    if ((a->batch * (a->head_q / a->head_k) / 64 + 2) * ((a->prefix_len + 127) / 128) * a->head_k > INT32_MAX)
+        return failf(DA_ERR_UNSUPPORTED, "batch * head_q * prefix_len is too large");
     if (a->rows < 0 || a->rows > INT32_MAX || a->prefix_rows < 0 || a->prefix_rows > INT32_MAX)
         return failf(DA_ERR_INVALID_ARG, "rows and prefix_rows must be in [0, 2^31)");
     if (!a->q || !a->o || !a->cu_seq_k) return failf(DA_ERR_INVALID_ARG, "q, o and cu_seq_k must not be NULL");

@@ -121,7 +121,8 @@ def test_prefix_arguments_are_refused(native_lib, change):
 def test_prefix_shapes_are_refused(native_lib):
     lib = native_lib.lib()
     for change in ({"dim": 256}, {"dim": 80}, {"head_q": 258}, {"prefix_table": PTR}, {"prefix_table": PTR, "prefix_page_size": 8},
-                   {"prefix_table": PTR, "prefix_page_size": 48}, {**PAGED, "page_size": 12}):
+                   {"prefix_table": PTR, "prefix_page_size": 48}, {**PAGED, "page_size": 12},
+                   {"batch": 65535, "head_q": 128, "prefix_table": PTR, "prefix_page_size": 64, "prefix_len": 1 << 30}):
         assert lib.da_prefix_decode_fwd(ctypes.byref(prefix_args(native_lib, **change))) == native_lib.DA_ERR_UNSUPPORTED
     assert lib.da_prefix_decode_fwd(None) == native_lib.DA_ERR_INVALID_ARG
 
