@@ -274,6 +274,12 @@ QuantCache check_cache(const at::Tensor &k, const at::Tensor &v, const at::Tenso
     return c;
 }
 
+// Rows whose elements lie side by side (a copy, if they do not).
+at::Tensor dense(const at::Tensor &x) { return x.dim() == 0 || x.stride(-1) == 1 ? x : x.contiguous(); }
+std::optional<at::Tensor> dense(const std::optional<at::Tensor> &x) {
+    return x.has_value() ? std::optional<at::Tensor>(dense(*x)) : std::nullopt;
+}
+
 void check_rows(const at::Tensor &x, const char *name, int64_t tokens, const QuantCache &c, const at::Device &device) {
     TORCH_CHECK(x.is_cuda() && x.device() == device, "all tensors must be on one CUDA device");
     TORCH_CHECK(x.dim() == 3 && x.size(0) == tokens && x.size(1) == c.head_k && x.size(2) == c.dim, name,
@@ -313,8 +319,9 @@ da_kv_rows_args_t rows_args(const at::Tensor &k, const at::Tensor &v, const at::
     return a;
 }
 
-void kv_cache_write(const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_cache, const at::Tensor &v_cache,
+void kv_cache_write(const at::Tensor &k_, const at::Tensor &v_, const at::Tensor &k_cache, const at::Tensor &v_cache,
                     const at::Tensor &k_scale, const at::Tensor &v_scale, std::optional<at::Tensor> slots) {
+    const at::Tensor k = dense(k_), v = dense(v_);
     TORCH_CHECK(k.dtype() == torch::kFloat16 || k.dtype() == torch::kBFloat16,
                 "Decoding-Attention only support FP16 and BF16 data type");
     TORCH_CHECK(v.dtype() == k.dtype(), "key and value must have the same dtype");
@@ -395,10 +402,11 @@ void check_table(const at::Tensor &table, int64_t batch, const at::Device &devic
 }
 int64_t row_stride(const at::Tensor &x) { return x.size(0) > 1 ? x.stride(0) : 0; }
 
-pybind11::object quantized_fwd(const at::Tensor &q, const at::Tensor &k_cache, const at::Tensor &v_cache,
+pybind11::object quantized_fwd(const at::Tensor &q_, const at::Tensor &k_cache, const at::Tensor &v_cache,
                                const at::Tensor &k_scale, const at::Tensor &v_scale, const at::Tensor &cu_seq_k,
                                bool is_alibi, std::optional<double> softmax_scale, std::optional<at::Tensor> out,
                                bool return_lse, std::optional<at::Tensor> block_table) {
+    const at::Tensor q = dense(q_);
     const QuantCache c = check_cache(k_cache, v_cache, k_scale, v_scale, q.device());
     check_cu(cu_seq_k, q.device());
     const int64_t batch = cu_seq_k.numel() - 1;
@@ -449,12 +457,15 @@ pybind11::object quantized_fwd(const at::Tensor &q, const at::Tensor &k_cache, c
     return pybind11::cast(r.o);
 }
 
-pybind11::object shared_prefix_fwd(const at::Tensor &q, const std::optional<at::Tensor> &k_prefix_,
-                                   const std::optional<at::Tensor> &v_prefix_, const at::Tensor &k, const at::Tensor &v,
+pybind11::object shared_prefix_fwd(const at::Tensor &q_, const std::optional<at::Tensor> &prefix_k,
+                                   const std::optional<at::Tensor> &prefix_v, const at::Tensor &own_k, const at::Tensor &own_v,
                                    const at::Tensor &cu_seq_k, bool is_alibi, std::optional<double> softmax_scale,
                                    std::optional<at::Tensor> out, bool return_lse, const std::optional<at::Tensor> &k_scale,
                                    const std::optional<at::Tensor> &v_scale, const std::optional<at::Tensor> &block_table,
                                    const std::optional<at::Tensor> &prefix_table, std::optional<int64_t> prefix_len) {
+    const at::Tensor q = dense(q_);
+    const std::optional<at::Tensor> k_prefix_ = dense(prefix_k), v_prefix_ = dense(prefix_v);
+    const at::Tensor k = k_scale.has_value() ? own_k : dense(own_k), v = k_scale.has_value() ? own_v : dense(own_v);
     const at::Device device = q.device();
     TORCH_CHECK(k_scale.has_value() == v_scale.has_value(), "k_scale and v_scale come together");
     TORCH_CHECK(k_prefix_.has_value() == v_prefix_.has_value(), "k_prefix and v_prefix come together");

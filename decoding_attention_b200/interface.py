@@ -91,7 +91,6 @@ def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots=None):
     A row whose a is below 2^-100 becomes zeros, a row with an infinity or a NaN reads back as NaN.
     The reference does not quantise its cache (README.md:154-156).
     """
-    k, v = [maybe_contiguous(x) for x in (k, v)]
     decoding_attn_cuda.kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots)
 
 
@@ -113,7 +112,6 @@ def quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, is_alibi=Fals
     ``block_table[b, j // page_size]`` (int32).  Keys whose row or page lies outside the cache are masked.  No length hint
     is needed: the work is divided on the device.  ``return_lse`` adds the fp32 natural-log LSE [batch, head_q].
     """
-    q = maybe_contiguous(q)
     return decoding_attn_cuda.quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, is_alibi, softmax_scale, out,
                                             return_lse, block_table)
 
@@ -132,8 +130,5 @@ def shared_prefix_fwd(q, k_prefix, v_prefix, k, v, cu_seq_k, is_alibi=False, sof
     codes with ``k_scale``, ``v_scale`` as ``kv_cache_write`` leaves them.  ALiBi counts positions through the prefix.
     ``return_lse`` adds the fp32 natural-log LSE [batch, head_q] over prefix and own keys.
     """
-    q, k_prefix, v_prefix = [maybe_contiguous(x) for x in (q, k_prefix, v_prefix)]
-    if k_scale is None:
-        k, v = [maybe_contiguous(x) for x in (k, v)]
     return decoding_attn_cuda.shared_prefix_fwd(q, k_prefix, v_prefix, k, v, cu_seq_k, is_alibi, softmax_scale, out, return_lse,
                                                 k_scale, v_scale, block_table, prefix_table, prefix_len)

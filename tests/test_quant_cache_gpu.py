@@ -380,6 +380,19 @@ def test_results_do_not_depend_on_what_else_is_in_the_batch_layout(api):
     assert (wide[:, 32:] == 3.0).all()
 
 
+def test_inputs_whose_elements_are_apart(api):
+    pr = problem("int8", torch.float16, [40, 0, 300], 8, 2, 64, 34)
+    o, _ = check(api, pr)
+    apart = torch.stack((pr["q"], torch.full_like(pr["q"], math.nan)), -1).flatten(-2)[..., ::2]
+    assert apart.stride(-1) == 2 and torch.equal(api.quantized_fwd(apart, pr["kc"], pr["vc"], pr["ks"], pr["vs"], pr["cu"]), o)
+    x = rows(7, 2, 64, torch.float16, 35)
+    a, b = [[torch.zeros(7, 2, 64, dtype=torch.int8, device=DEV) for _ in range(2)] + [torch.zeros(7, 2, device=DEV) for _ in range(2)]
+            for _ in range(2)]
+    api.kv_cache_write(x, 2 * x, *a)
+    api.kv_cache_write(torch.stack((x, x), -1)[..., 0], x.transpose(0, 2).contiguous().transpose(0, 2) * 2, *b)
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
 def test_two_streams_and_graph_replay(api):
     pr = problem("int8", torch.bfloat16, [513, 4000, 0, 9, 77], 32, 8, 128, 24)
     args = (pr["q"], pr["kc"], pr["vc"], pr["ks"], pr["vs"], pr["cu"])
