@@ -319,12 +319,12 @@ PrefixGrid plan_prefix(int sms, int batch, int head_k, int group, int prefix_len
 
 // What a key of the sequences' own costs an SM, in 1/65536 of a key tile of the prefix; 0 where the prefix does not fill the
 // SMs anyway.  Measured: a key tile of two row tiles takes an SM 2.6 us at dim 128, an SM alone streams 54 GB/s of 16-bit
-// rows, and no format goes below 7 ns for a key and KV head of 128 columns and eight query heads.
+// rows, and codes take 7 (int8), 8 (FP8) or 9 ns (int4) for a key and KV head of 128 columns and eight query heads.
 int own_cost(const StreamParams &s, const PrefixGrid &g, int dim, int kind) {
     if (g.total < 2 * g.sms) return 0;
     const double tile = (dim <= 64 ? 1800.0 : 2600.0) * g.row_tiles / (2 * g.pairs);
     const double bytes = kind == DA_KV_SAME_AS_Q ? 4.0 * dim : (kind == DA_KV_INT4 ? 1.0 : 2.0) * dim + 8;
-    const double memory = bytes / 54.0, work = 7.0 * ((s.group + 7) / 8) * dim / 128;
+    const double memory = bytes / 54.0, work = (kind == DA_KV_FP8_E4M3 ? 8.0 : (kind == DA_KV_INT4 ? 9.0 : 7.0)) * ((s.group + 7) / 8) * dim / 128;
     const double share = s.head_k * (memory > work ? memory : work) / tile * 65536.0;
     return share < 1.0 ? 1 : (share > 1e9 ? 1000000000 : (int)share);
 }
@@ -370,6 +370,8 @@ PrefixPlan fill_prefix(const da_prefix_decode_args_t *a, int sms, StreamParams *
     if (a->prefix_len > 0) {
         plan.grid = plan_prefix(sms, s->batch, s->head_k, s->group, (int)a->prefix_len);
         plan.grid.own_cost = own_cost(*s, plan.grid, (int)a->dim, a->kv_dtype);
+        plan.grid.most_tiles = (int)(((int64_t)plan.grid.total * 4 + sms - 1) / sms);
+        plan.grid.by_sms = ~0ull / ((unsigned long long)sms << 16) + 1;
         if (plan.grid.own_cost) s->beside = plan.grid;
         plan.parts = ((size_t)plan.grid.max_parts * rows * row + 3) / 4 * 4;
         plan.own = (rows * row + 3) / 4 * 4;

@@ -25,16 +25,22 @@ struct PrefixGrid {
     // the key stream.  How many own keys there are is known on the device only.
     int own_cost;    // of an own key, in 1/65536 of a key tile's; 0: no sharing
     int sms;
+    int most_tiles;             // of a CTA then: the prefix keeps a quarter of the SMs
+    unsigned long long by_sms;  // 2^64 / (65536 sms), rounded up
 };
-constexpr int kShareTiles = 4;  // the prefix keeps a quarter of the SMs
 
-// Key tiles of a CTA next to so many own keys (the same in all three kernels of a call).
+// Key tiles of a CTA next to so many own keys (the same in all three kernels of a call, and on the way to their first load:
+// no 64-bit division).
 __host__ __device__ inline int prefix_run(const PrefixGrid &g, long long keys) {
-    const long long prefix = (long long)g.total << 16, own = keys * g.own_cost;
+    const unsigned long long prefix = (unsigned long long)g.total << 16, own = (unsigned long long)keys * (unsigned)g.own_cost;
     if (own < prefix / 8) return g.cta_tiles;  // (not worth the longer runs: 170 us instead of 166 with 9 % of own work)
-    const long long run = (prefix + own) / ((long long)g.sms << 16) + 1;
-    const long long most = ((long long)g.total * kShareTiles + g.sms - 1) / g.sms;
-    return (int)(run > most ? most : (run < g.cta_tiles ? g.cta_tiles : run));
+#ifdef __CUDA_ARCH__
+    const long long even = (long long)__umul64hi(prefix + own, g.by_sms);
+#else
+    const long long even = (long long)(((unsigned __int128)(prefix + own) * g.by_sms) >> 64);
+#endif
+    // (rounded down: a run's start and end take about a tile longer than a span's)
+    return even > g.most_tiles ? g.most_tiles : (even < g.cta_tiles ? g.cta_tiles : (int)even);
 }
 
 struct PrefixParams {

@@ -101,8 +101,8 @@ __device__ __forceinline__ SpanPlan span_plan(const StreamParams &p) {
     if (p.beside.own_cost) {
         // As many spans as the SMs that the prefix leaves free take in whole waves.
         const int run = prefix_run(p.beside, keys > 0 ? keys : 0);
-        const int left = p.beside.sms - (p.beside.total + run - 1) / run;
-        if (run > p.beside.cta_tiles && left > 0) spans = (int)((long long)spans * (p.beside.sms / left * left) / p.beside.sms);
+        const unsigned sms = p.beside.sms, left = sms - ((unsigned)p.beside.total + run - 1) / (unsigned)run;
+        if (run > p.beside.cta_tiles && left > 0) spans = (int)((unsigned)spans * (sms / left * left) / sms);
         if (spans < 1) spans = 1;
     }
     long long units = axis_div(s.total + spans - 1, spans);
