@@ -17,9 +17,11 @@
 // instead of assuming packed rows (decoding_attn.cpp:32-46), and library errors raise instead of
 // terminating the process.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <array>
 #include <cstring>
 #include <optional>
 #include <tuple>
@@ -353,8 +355,10 @@ std::tuple<at::Tensor, at::Tensor> kv_cache_read(const at::Tensor &k_cache, cons
         check_rows(k, "out[0]", tokens, c, device);
         check_rows(v, "out[1]", tokens, c, device);
     } else {
-        k = torch::empty({tokens, c.head_k, c.dim}, k_cache.options().dtype(dtype));
-        v = torch::empty({tokens, c.head_k, c.dim}, k_cache.options().dtype(dtype));
+        // (all of it is written, and the call is short: straight to the allocator)
+        const std::array<int64_t, 3> shape = {tokens, c.head_k, c.dim};
+        k = at::detail::empty_cuda(shape, dtype, device, std::nullopt);
+        v = at::detail::empty_cuda(shape, dtype, device, std::nullopt);
     }
     da_kv_rows_args_t a = rows_args(k, v, k_cache, v_cache, k_scale, v_scale, c);
     a.slots = check_slots(slots, tokens, device);
