@@ -175,6 +175,21 @@ def test_own_keys_next_to_a_long_prefix(api, hq, hk, dim, batch, kind):
         check(api, problem(torch.bfloat16, prefix, lens, hq, hk, dim, 30, kind=kind, page=page), alibi=top == 900, what=f"{kind} {top}")
 
 
+def test_two_streams_with_work_for_all_sms(api):
+    """Calls that divide the SMs, next to one another and to calls with codes: each result is that of the call alone."""
+    prs = [problem(torch.bfloat16, 3000, [(i * 41) % 700 for i in range(90)], 32, 8, 128, 32 + j, kind=kind)
+           for j, kind in enumerate((None, "fp8"))]
+    want = [check(api, pr) for pr in prs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for turn in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append(((turn + i) % 2, call(api, prs[(turn + i) % 2])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[j][0]) and torch.equal(lse, want[j][1]) for j, (o, lse) in got)
+
+
 def test_replay_with_other_lengths(api):
     """A captured call is used with lengths that change which SMs do what."""
     batch, hq, hk, dim, prefix = 70, 32, 8, 128, 2500
