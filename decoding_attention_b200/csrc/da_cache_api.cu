@@ -118,10 +118,13 @@ void plan_stream(int dim, int kind, int sms, StreamParams *p) {
     const int blocks = (streams + p->head_warps - 1) / p->head_warps;
     const int slots = sms * shape.ctas_per_sm;
     p->spans = slots > blocks ? slots / blocks : 1;
-    // A piece of a sequence costs a CTA about as long as 16 keys of a warp, however short it is (its queries, the joining of
-    // its warps, its output); a CTA gets at least twice as much again to do.
-    p->piece_cost = 16 * p->key_warps;
-    p->min_span = 48 * p->key_warps;
+    // A piece of a sequence costs a CTA about as long as 64 keys of a warp, however short it is (its queries, the joining of
+    // its warps, its output), and a span is longer than that.  With few sequences the spans' shortest length matters more
+    // than their balance: half as much then.  (32 x 1 024-4 096 int4 keys, 32/2 heads: 24.7 us with a cost of 16, 23.5 with
+    // 32, 22.6 with 64; 4 x 500-2 000, 32/8 heads: 13.9, 13.2 and 15.4.)
+    const int cost = p->batch >= 16 ? 64 : 32;
+    p->piece_cost = cost * p->key_warps;
+    p->min_span = (cost + 32) * p->key_warps;
 }
 
 size_t stream_piece_bytes(const StreamParams &p, int dim) {
