@@ -276,8 +276,11 @@ QuantCache check_cache(const at::Tensor &k, const at::Tensor &v, const at::Tenso
     return c;
 }
 
-// Rows whose elements lie side by side (a copy, if they do not).
-at::Tensor dense(const at::Tensor &x) { return x.dim() == 0 || x.stride(-1) == 1 ? x : x.contiguous(); }
+// Whether rows [tokens, heads, dim] share memory, as those of a tensor expanded over its tokens do (row stride 0, which
+// the library takes for packed rows).
+bool rows_overlap(const at::Tensor &x) { return x.dim() == 3 && x.size(0) > 1 && x.stride(0) < x.size(1) * x.size(2); }
+// Rows that do not overlap, with their elements side by side: a copy, if they are not like that.
+at::Tensor dense(const at::Tensor &x) { return x.dim() == 0 || (x.stride(-1) == 1 && !rows_overlap(x)) ? x : x.contiguous(); }
 std::optional<at::Tensor> dense(const std::optional<at::Tensor> &x) {
     return x.has_value() ? std::optional<at::Tensor>(dense(*x)) : std::nullopt;
 }
@@ -287,6 +290,7 @@ void check_rows(const at::Tensor &x, const char *name, int64_t tokens, const Qua
     TORCH_CHECK(x.dim() == 3 && x.size(0) == tokens && x.size(1) == c.head_k && x.size(2) == c.dim, name,
                 " must have shape (tokens, head_k, dim) with the caches' head_k and dim");
     TORCH_CHECK(x.stride(2) == 1 && (c.head_k == 1 || x.stride(1) == c.dim), "heads must be contiguous inside a token row");
+    TORCH_CHECK(!rows_overlap(x), name, " must have rows of its own for every token");
 }
 
 const int64_t *check_slots(const std::optional<at::Tensor> &slots, int64_t tokens, const at::Device &device) {
@@ -387,6 +391,7 @@ Outputs make_outputs(const at::Tensor &q, const std::optional<at::Tensor> &out, 
         TORCH_CHECK(r.o.is_cuda() && r.o.device() == q.device(), "all tensors must be on one device");
         TORCH_CHECK(r.o.sizes() == q.sizes(), "out must have the shape of the query");
         TORCH_CHECK(r.o.stride(2) == 1 && (q.size(1) == 1 || r.o.stride(1) == q.size(2)), "heads must be contiguous inside a token row");
+        TORCH_CHECK(!rows_overlap(r.o), "out must have rows of its own for every sequence");
     } else {
         r.o = torch::empty(q.sizes(), q.options());
     }

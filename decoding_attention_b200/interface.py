@@ -89,6 +89,7 @@ def kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots=None):
 
     With a = max |x| of a row and Q = 448, 127 or 7: scale = a / Q, code = x * (Q / a) to the nearest, ties to even.
     A row whose a is below 2^-100 becomes zeros, a row with an infinity or a NaN reads back as NaN.
+    k and v may be expanded over their tokens, like the inputs of the calls below (they are copied first); an ``out`` may not.
     The reference does not quantise its cache (README.md:154-156).
     """
     decoding_attn_cuda.kv_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots)
