@@ -40,10 +40,16 @@ struct Outputs {
     at::Tensor lse;
 };
 
-Outputs run(const at::Tensor &q, const at::Tensor &k, const std::optional<at::Tensor> &v_,
+// Whether rows [tokens, heads, dim] share memory, as those of a tensor expanded over its tokens do (row stride 0, which
+// the library takes for packed rows).
+bool rows_overlap(const at::Tensor &x) { return x.dim() == 3 && x.size(0) > 1 && x.stride(0) < x.size(1) * x.size(2); }
+at::Tensor own_rows(const at::Tensor &x) { return rows_overlap(x) ? x.contiguous() : x; }
+
+Outputs run(const at::Tensor &q_, const at::Tensor &k_, const std::optional<at::Tensor> &v_,
             const std::optional<at::Tensor> &o_, const at::Tensor &cu_seq_k, int64_t max_seq_k, int64_t dim_v,
             bool is_alibi, std::optional<double> softmax_scale, bool want_lse, const at::Tensor *block_table = nullptr,
             int64_t page_size = 0, double k_scale = 1.0, double v_scale = 1.0) {
+    const at::Tensor q = own_rows(q_), k = own_rows(k_);
     auto q_dtype = q.dtype();
     TORCH_CHECK(q_dtype == torch::kFloat16 || q_dtype == torch::kBFloat16,
                 "Decoding-Attention only support FP16 and BF16 data type");
@@ -96,8 +102,9 @@ Outputs run(const at::Tensor &q, const at::Tensor &k, const std::optional<at::Te
     a.q_row_stride = q.stride(0);
     a.k_row_stride = k.stride(0);
 
+    at::Tensor v;  // (kept until the launch: it may be a copy)
     if (v_.has_value()) {
-        const at::Tensor &v = v_.value();
+        v = own_rows(v_.value());
         TORCH_CHECK(v.dtype() == k.dtype(), fp8_cache ? "key and value must have the same quantised dtype" : "query and value must have the same dtype");
         DA_CHECK_DEVICE(v);
         TORCH_CHECK(v.device() == q.device(), "all tensors must be on one device");
@@ -117,6 +124,7 @@ Outputs run(const at::Tensor &q, const at::Tensor &k, const std::optional<at::Te
         TORCH_CHECK(out.o.stride(-1) == 1, "Output tensor must have contiguous last dimension");
         DA_CHECK_SHAPE(out.o, total_q, head_q, dim_v);
         TORCH_CHECK(out.o.stride(1) == dim_v, "heads must be contiguous inside a token row");
+        TORCH_CHECK(!rows_overlap(out.o), "Output tensor must have rows of its own for every sequence");
     } else {
         out.o = torch::empty({total_q, head_q, dim_v}, q.options());
     }
@@ -276,9 +284,6 @@ QuantCache check_cache(const at::Tensor &k, const at::Tensor &v, const at::Tenso
     return c;
 }
 
-// Whether rows [tokens, heads, dim] share memory, as those of a tensor expanded over its tokens do (row stride 0, which
-// the library takes for packed rows).
-bool rows_overlap(const at::Tensor &x) { return x.dim() == 3 && x.size(0) > 1 && x.stride(0) < x.size(1) * x.size(2); }
 // Rows that do not overlap, with their elements side by side: a copy, if they are not like that.
 at::Tensor dense(const at::Tensor &x) { return x.dim() == 0 || (x.stride(-1) == 1 && !rows_overlap(x)) ? x : x.contiguous(); }
 std::optional<at::Tensor> dense(const std::optional<at::Tensor> &x) {

@@ -1,5 +1,5 @@
 """GPU tests of tensors whose rows share memory (expanded over tokens or sequences): inputs give what their copies give,
-outputs are refused."""
+outputs are refused.  The unquantised calls are held to the same."""
 import pytest
 import torch
 
@@ -101,3 +101,42 @@ def test_outputs_whose_rows_overlap_are_refused(api):
     # one row overlaps with none, whatever its stride
     o = torch.empty(8, 128, dtype=torch.bfloat16, device=DEV).as_strided((1, 8, 128), (0, 128, 1))
     assert torch.equal(api.quantized_fwd(q[:1], *caches, cu[:2], out=o), api.quantized_fwd(q[:1], *caches, cu[:2]))
+
+
+def copied(x):
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+@pytest.mark.parametrize("hq,hk", [(8, 8), (16, 4), (32, 1)])
+def test_unquantised_calls_with_expanded_inputs(api, hq, hk):
+    lens = [40, 0, 300, 7, 1]
+    n, batch, dim = sum(lens), len(lens), 128
+    cu = torch.tensor([0] + lens, device=DEV).cumsum(0).to(torch.int32)
+    q, k, v = rand(batch, hq, dim, seed=1), rand(n, hk, dim, seed=2), rand(n, hk, dim, seed=3)
+    for x in one_and_overlapping(batch, hq, dim, 4):
+        assert torch.equal(api.dmha_fwd(x, k, v, cu, 300), api.dmha_fwd(copied(x), k, v, cu, 300))
+        assert torch.equal(api.decoding_attn_fwd(x, k, v, cu, 300, dim, False), api.dmha_fwd(copied(x), k, v, cu, 300))
+    for a, b in zip(one_and_overlapping(n, hk, dim, 5), one_and_overlapping(n, hk, dim, 6)):
+        assert torch.equal(api.dmha_fwd(q, a, b, cu, 300), api.dmha_fwd(q, copied(a), copied(b), cu, 300))
+    table = torch.arange(batch * 20, device=DEV).to(torch.int32).view(batch, 20)
+    pools = rand(batch * 20, 16, hk, dim, seed=7), rand(batch * 20, 16, hk, dim, seed=8)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for x in one_and_overlapping(batch, hq, dim, 9):
+        assert torch.equal(api.paged_fwd(x, *pools, lengths, table), api.paged_fwd(copied(x), *pools, lengths, table))
+    for bad in one_and_overlapping(batch, hq, dim, 10):
+        with pytest.raises(RuntimeError, match="rows of its own"):
+            api.dmha_fwd(q, k, v, cu, 300, out=bad)
+        with pytest.raises(RuntimeError, match="rows of its own"):
+            api.paged_fwd(q, *pools, lengths, table, out=bad)
+
+
+def test_latent_cache_with_expanded_inputs(api):
+    cu = torch.tensor([0, 50, 50, 90], dtype=torch.int32, device=DEV)
+    q, kv = rand(3, 16, 576, seed=1), rand(90, 1, 576, seed=2)
+    for x in one_and_overlapping(3, 16, 576, 3):
+        assert torch.equal(api.dmla_fwd(x, kv, cu, 50), api.dmla_fwd(copied(x), kv, cu, 50))
+    for x in one_and_overlapping(90, 1, 576, 4):
+        assert torch.equal(api.dmla_fwd(q, x, cu, 50), api.dmla_fwd(q, copied(x), cu, 50))
+    for bad in one_and_overlapping(3, 16, 512, 5):
+        with pytest.raises(RuntimeError, match="rows of its own"):
+            api.dmla_fwd(q, kv, cu, 50, out=bad)
