@@ -152,6 +152,13 @@ da_prefix_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap tm_q,
         }
         const int run = p.table && (1 << p.page_shift) < kKeys ? 1 << p.page_shift : kKeys;
         const uint32_t q_bytes = (uint32_t)(C::kBlocks * 128 * p.group * g.tile_seqs);
+        // Row of a key; rows of a page that is not in the pool are fetched from in front of the map, i.e. as zeros.
+        auto row_of = [&](int key) -> int {
+            if (!p.table) return key;
+            const int page = p.table[key >> p.page_shift];
+            const long long row = ((long long)page << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+            return page < 0 || row >= p.rows ? -kKeys : (int)row;
+        };
         int fill = 0;  // tiles staged so far, K and V counted apart
         int pieces = 0;
         for (long long at = begin; ok && x.load(g, at, end); at = x.next, ++pieces) {
@@ -180,7 +187,7 @@ da_prefix_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap tm_q,
                             mbar_arrive_expect_tx(&slot_full[st], C::kTileBytes);
                             for (int k0 = 0; k0 < kKeys; k0 += run) {
                                 const int key = key0 + k0;
-                                const int row = p.table ? (p.table[key >> p.page_shift] << p.page_shift) + (key & ((1 << p.page_shift) - 1)) : key;
+                                const int row = row_of(key);
                                 for (int kb = 0; kb < C::kBlocks; ++kb)
                                     tma_load_tile_3d(dst + kb * kBlockBytes + k0 * 128, kv ? &tm_v : &tm_k, kb * 64, x.hk, row, &slot_full[st]);
                             }
