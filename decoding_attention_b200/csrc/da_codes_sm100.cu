@@ -38,6 +38,9 @@ constexpr int kCtas = 3;                // per SM
 constexpr int kSoftmaxThreads = 128;
 constexpr int kThreads = 256;           // (the last warp only fills up)
 constexpr float kHeadroom = 1.0f;       // log2 of what a score or weight may exceed its reference by
+// log2 of how far the weights' reference may lie below the scores': the leading keys' V scales may be zero, and 2^(m - mw)
+// has to stay a number.  Weights 2^-120 of a probability of one are far below what o can show.
+constexpr float kWeightReach = 120.0f;
 constexpr int kFlushTiles = 256;        // 32 768 keys: int32 holds 66 311 of 127 * 255
 // Tiles of K and V, in turn.  Even, so that a slot is K's or V's for good: with an odd number the K issuer, which may be
 // three tiles ahead of the other, could wait for a phase of a slot whose previous phase (a V tile) is still under way --
@@ -457,7 +460,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                             c = fmaxf(c, y.y);
                         }
                         l[h] *= exp2f(m0 - a);
-                        shrink[h] = exp2f(mw0 - c);
+                        shrink[h] = exp2f(mw0 - fmaxf(c, a - kWeightReach));
                         s[h] = valid ? s[h] : -INFINITY;
                     }
                     named_bar_sync(2, kSoftmaxThreads);
@@ -469,9 +472,10 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                             a = fmaxf(a, y.x);
                             c = fmaxf(c, y.y);
                         }
+                        c = fmaxf(c, a - kWeightReach);
                         hs[tid].m = a;
                         hs[tid].mw = c;
-                        hs[tid].g = c > -1e29f ? exp2f(a - c) : 1.0f;  // (no weight so far: all V scales are zero)
+                        hs[tid].g = exp2f(a - c);
                     }
                     if (since > 0) {  // the last contraction has finished: take over what it has
                         ok &= (bool)__all_sync(0xffffffffu, mbar_wait(&p_empty[(t - 1) & 1], (uint32_t)((t - 1) >> 1) & 1u, abort_flag));
@@ -499,7 +503,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                     for (int e = 0; e < 2; ++e) {
                         const float pr = exp2f(s[h + e] - hs[h + e].m);
                         l[h + e] += pr;
-                        w[e] = pr * (scaled_vs * hs[h + e].g);
+                        w[e] = (pr * hs[h + e].g) * scaled_vs;  // (in this order: vs g alone may be past fp32)
                     }
                     if (kInt) {
 #pragma unroll
@@ -563,7 +567,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                 if (h >= heads) break;
                 const float sum = red[h].x + red[kHeads + h].x + red[2 * kHeads + h].x + red[3 * kHeads + h].x;
                 // o is in units of 2^mw, the sum in units of 2^m
-                const float v = (sum > 0.0f ? o[h] * (1.0f / (sum * hs[h].g)) : (sum == 0.0f ? 0.0f : sum)) + odd;
+                const float v = (sum > 0.0f ? o[h] * (1.0f / sum) * (1.0f / hs[h].g) : (sum == 0.0f ? 0.0f : sum)) + odd;
                 const long long out = (long long)x.b * p.head_q + head0 + h;
                 const long long piece = (span * 2 + (x.begin == 0 ? 1 : 0)) * p.head_q + head0 + h;
                 const float lse = sum == 0.0f ? -INFINITY : (hs[h].m + log2f(sum)) * kLn2;

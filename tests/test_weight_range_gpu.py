@@ -1,0 +1,96 @@
+"""GPU tests of decode attention where softmax weights and V scales differ by many powers of two: a key that takes nearly
+all of the weight next to many that share the rest, V rows of zeros, V rows of any size."""
+import math
+
+import pytest
+import torch
+
+import quant_reference as ref
+import weight_bounds
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+KINDS = ["fp8", "int8", "int4"]
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def api():
+    import decoding_attention_b200
+    return decoding_attention_b200
+
+
+def cache_of(n, hk, dim, kind, seed, k_spread=0.1):
+    """Codes and scales of a sequence whose scores stay small: K rows of about 0.05, V rows of about one."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    out = []
+    for size in (0.05, 1.0):
+        x = size * torch.randn(n, hk, dim, device=DEV, generator=g) + (0.5 if size == 1.0 else 0.0)
+        codes, s = ref.quantise(x, kind)
+        out += [codes, s]
+    return out
+
+
+def raise_key(q, k_code, k_scale, j, nats):
+    """Gives key j a score of about `nats` in all heads (q is the same in all of them)."""
+    row = q[0].double()
+    top = 112.0 if k_code.abs().max() > 7 else 7.0
+    code = torch.round(row / row.abs().max() * top)
+    # (numbers that e4m3 has too)
+    code = torch.where(code.abs() > 16, torch.round(code / 16) * 16, code) if top == 112.0 else code
+    k_code[j] = code
+    k_scale[j] = nats * math.sqrt(len(row)) / float(row @ code)
+
+
+def run(api, q, parts, kind, alibi=False, softmax_scale=None):
+    k_code, k_scale, v_code, v_scale = parts
+    cu = torch.tensor([0, len(k_code)], dtype=torch.int32, device=DEV)
+    return api.quantized_fwd(q[None], ref.pack(k_code, kind), ref.pack(v_code, kind), k_scale.float(), v_scale.float(), cu,
+                             is_alibi=alibi, softmax_scale=softmax_scale, return_lse=True)
+
+
+def check(api, q, parts, kind, alibi=False, softmax_scale=None, what=""):
+    parts = [parts[0], parts[1].float(), parts[2], parts[3].float()]
+    o, lse = run(api, q, parts, kind, alibi, softmax_scale)
+    found = weight_bounds.attend(q, *parts, alibi=alibi, softmax_scale=softmax_scale)
+    tol, tol_lse = weight_bounds.bounds(found, len(parts[0]), 11, o.dtype)
+    assert ((lse[0].double() - found["lse"]).abs() <= tol_lse).all(), f"{what} lse: off by {(lse[0].double() - found['lse']).abs().max()}"
+    over = (o[0].double() - found["o"]).abs() / tol
+    assert (over <= 1.0).all(), f"{what}: {over.max().item():.3g} of the bound"  # (NaN is over it)
+
+
+def query(hq, dim, dtype, seed=5):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randn(1, dim, device=DEV, generator=g).to(dtype).expand(hq, -1).contiguous()
+
+
+@pytest.mark.parametrize("hq,hk,dim", [(8, 2, 128), (8, 8, 96)])
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+def test_the_leading_key_has_a_v_row_of_zeros(api, kind, hq, hk, dim):
+    """By so much that the weights of all others are below what fp32 holds, and by less."""
+    q = query(hq, dim, torch.bfloat16)
+    for nats in (200.0, 95.0, 82.0, 60.0):
+        for n in (300, 3000):
+            for j in (0, 130, n - 1):
+                parts = cache_of(n, hk, dim, kind, 6)
+                raise_key(q, parts[0], parts[1], j, nats)
+                parts[2][j], parts[3][j] = 0.0, 0.0
+                check(api, q, parts, kind, what=f"{kind} {hq}/{hk} {dim} {nats} nats, {n} keys, key {j}")
+
+
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+def test_zero_v_rows_at_the_end_under_alibi(api, kind):
+    hq, hk, dim, n = 8, 2, 128, 700
+    parts = cache_of(n, hk, dim, kind, 7)
+    parts[2][-300:], parts[3][-300:] = 0.0, 0.0
+    check(api, query(hq, dim, torch.bfloat16), parts, kind, alibi=True, what=kind)
+
+
+def test_all_v_rows_are_zeros(api):
+    for kind in KINDS:
+        parts = cache_of(400, 2, 128, kind, 8)
+        parts[2].zero_()
+        parts[3].zero_()
+        q = query(8, 128, torch.float16)
+        check(api, q, parts, kind, what=kind)
+        assert (run(api, q, parts, kind)[0] == 0).all()
