@@ -22,10 +22,12 @@
 // CTA an SM that fits: 191 us for the int4 case above); and 32 heads a warp, so that a group of 32 is widened once instead
 // of twice (128 sequences of 2 048 int4 keys, 32 heads over one KV head: 51 us, 42 with two warps of 16 heads).
 //
-// q is brought to fp16 with a power of two per head that makes its largest element 1..2 (exact; undone in the score's
-// factor), whatever its own type.  The weights w_j = p_j vs_j are rounded to fp16 after a second factor per head, kept
-// like the reference maximum, has brought their running maximum near 1: half a step of fp16, 2^-11, is the only rounding
-// between q and o, and sums, maxima and outputs are fp32.
+// q is brought to fp16 with a power of two per head that makes its largest element 1..2, undone in the score's factor:
+// exact, but for elements of a bf16 head below 2^-14 of its largest, which keep 2^-25 of that.  The weights w_j = p_j vs_j
+// are rounded to fp16 in units of their own, a power of two per head that is kept like the reference maximum: the largest
+// weight so far comes to 2^7..2^15, so that a weight is off by half a step, 2^-11 of itself, or by 2^-32 of the largest.
+// (The units follow the weights and not the probabilities: a key that leads by far may have a V row of zeros.)  Between q
+// and o these are the only roundings to fewer bits; sums, maxima and outputs are fp32.
 //
 // Work split.  Lengths live on the device, so the CTAs cut the concatenated keys of the whole batch into equal spans
 // (StreamParams): any mix of lengths keeps all SMs busy to the end, without a sort or a guess of the longest sequence.
@@ -97,6 +99,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// The power of two at or below a positive number (-127: none that is normal), and back.
+__device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }
+__device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+constexpr int kMostScaled = 100;  // log2 of what a V scale may come to in the units of the weights
 
 // ---- codes to pairs of fp16 --------------------------------------------------------------------
 __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
@@ -531,6 +538,15 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[t][n][e] = 0.0f;
 
+        // Units of the weights: f a head, f_top the largest of this lane's heads.
+        uint32_t unset = 0;  // heads whose reference maximum has risen, but no weight come since (a bit each, the same in a column's lanes)
+        float f_top = 1.0f;
+        auto set_f_top = [&]() {
+            f_top = f[0][0];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) f_top = fmaxf(f_top, fmaxf(f[n][0], f[n][1]));
+        };
+
         const int tiles = idle ? 0 : tiles_of(con);
         for (int step = 0; step < tiles; ++step) {
             const int key0 = tile_key(con, step, tiles);
@@ -564,7 +580,6 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
             }
             // ---- scale, bias, mask; is a new reference maximum due? ----
             bool raise = false;
-            uint32_t fresh = 0;  // heads whose largest score so far is in this tile (one bit each, the same in all lanes of a column)
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -608,7 +623,18 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                     for (int t = 0; t < MT; ++t) top = fmaxf(top, fmaxf(s[t][n][e], s[t][n][2 + e]));
                     raise |= top > m[n][e] + 8.0f;
                 }
+            // New units for the weights too, where V rows far larger than those before would leave fp32 in the old ones.
+            float v_top = 0.0f;
+            if (C::kQuant) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) v_top = fmaxf(v_top, fmaxf(sc[TK + t * 16 + key_r], sc[TK + t * 16 + 8 + key_r]));
+                raise |= v_top * f_top > power2(kMostScaled);
+            }
             if (__any_sync(0xffffffffu, raise)) {
+                if (C::kQuant) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, d));
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -618,13 +644,19 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                         for (int t = 0; t < MT; ++t) top = fmaxf(top, fmaxf(s[t][n][e], s[t][n][2 + e]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const float shrink = exp2_fast(m[n][e] - top);
-                        if (top > m[n][e]) fresh |= 1u << (2 * n + e);
+                        float shrink = exp2_fast(m[n][e] - top);
+                        if (top > m[n][e]) unset |= 1u << (2 * n + e);
                         m[n][e] = top;
                         l[n][e] *= shrink;
+                        if (C::kQuant) {
+                            const int by = min(0, kMostScaled - exponent(v_top) - exponent(f[n][e]));
+                            f[n][e] = power2(exponent(f[n][e]) + by);
+                            shrink *= power2(max(-126, by));  // (past that there is nothing to keep)
+                        }
 #pragma unroll
                         for (int t = 0; t < C::MTILES; ++t) acc[t][n][e] *= shrink, acc[t][n][2 + e] *= shrink;
                     }
+                set_f_top();
             }
             // ---- probabilities, weights ----
             bool wide = false;
@@ -641,15 +673,16 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                             l[n][e] += pr;
                             if (C::kQuant) {
                                 s[t][n][2 * g + e] = pr * (vs * f[n][e]);
-                                wide |= s[t][n][2 * g + e] > 512.0f;
+                                wide |= s[t][n][2 * g + e] > 32768.0f;
                             } else {
                                 s[t][n][2 * g + e] = pr;
                             }
                         }
                 }
-            if (C::kQuant && (__any_sync(0xffffffffu, wide || raise))) {
-                // The weights' own reference: the largest of this tile comes to 1..2 if it has outgrown its units, or if
-                // its head's largest probability is in this tile (then a small weight may be the one that matters).
+            if (C::kQuant && (__any_sync(0xffffffffu, wide || unset != 0))) {
+                // The weights' own reference: the largest of this tile comes to 2^7..2^8 if it has outgrown its units, or if
+                // it is the first that is not zero since the reference maximum rose (a small weight may then be the one that
+                // matters) -- as far as what has been summed up so far still fits fp32.
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -659,16 +692,25 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                         for (int t = 0; t < MT; ++t) top = fmaxf(top, fmaxf(s[t][n][e], s[t][n][2 + e]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const int ex = (int)(__float_as_uint(top) >> 23);
-                        if (ex > 1 && ex < 253 && (ex > 127 || ((fresh >> (2 * n + e)) & 1u))) {
-                            const float g = __uint_as_float((uint32_t)(254 - ex) << 23);
-                            f[n][e] *= g;
+                        float held = 0.0f;
+#pragma unroll
+                        for (int t = 0; t < C::MTILES; ++t) held = fmaxf(held, fmaxf(fabsf(acc[t][n][e]), fabsf(acc[t][n][2 + e])));
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) held = fmaxf(held, __shfl_xor_sync(0xffffffffu, held, d));
+                        const int ex = exponent(top);
+                        if (ex > -127 && ex < 128 && (ex >= 15 || ((unset >> (2 * n + e)) & 1u))) {
+                            unset &= ~(1u << (2 * n + e));
+                            // (no less than -102: a V scale is at most 2^101 in these units, a probability 2^8)
+                            const int by = min(min(min(7 - ex, 126), 120 - exponent(f[n][e])), max(0, 100 - exponent(held)));
+                            const float g = power2(by);
+                            f[n][e] = power2(exponent(f[n][e]) + by);
 #pragma unroll
                             for (int t = 0; t < MT; ++t) s[t][n][e] *= g, s[t][n][2 + e] *= g;
 #pragma unroll
                             for (int t = 0; t < C::MTILES; ++t) acc[t][n][e] *= g, acc[t][n][2 + e] *= g;
                         }
                     }
+                set_f_top();
             }
             // ---- output ----
 #pragma unroll

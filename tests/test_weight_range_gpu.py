@@ -11,6 +11,9 @@ import weight_bounds
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 KINDS = ["fp8", "int8", "int4"]
+# Formats and head layouts: codes as tensor-core operands, codes widened in registers.
+CODES = [("fp8", 8, 2, 128), ("int8", 8, 2, 128), ("fp8", 8, 8, 96), ("int8", 8, 8, 96)]
+STREAM = [("int4", 8, 2, 128), ("int4", 32, 1, 96), ("int8", 8, 2, 64), ("int8", 32, 2, 128), ("fp8", 4, 1, 256), ("fp8", 16, 1, 64)]
 DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
 
 
@@ -64,12 +67,11 @@ def query(hq, dim, dtype, seed=5):
     return torch.randn(1, dim, device=DEV, generator=g).to(dtype).expand(hq, -1).contiguous()
 
 
-@pytest.mark.parametrize("hq,hk,dim", [(8, 2, 128), (8, 8, 96)])
-@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("kind,hq,hk,dim", CODES + STREAM)
 def test_the_leading_key_has_a_v_row_of_zeros(api, kind, hq, hk, dim):
     """By so much that the weights of all others are below what fp32 holds, and by less."""
     q = query(hq, dim, torch.bfloat16)
-    for nats in (200.0, 95.0, 82.0, 60.0):
+    for nats in (200.0, 95.0, 82.0, 60.0, 12.0):
         for n in (300, 3000):
             for j in (0, 130, n - 1):
                 parts = cache_of(n, hk, dim, kind, 6)
@@ -78,9 +80,9 @@ def test_the_leading_key_has_a_v_row_of_zeros(api, kind, hq, hk, dim):
                 check(api, q, parts, kind, what=f"{kind} {hq}/{hk} {dim} {nats} nats, {n} keys, key {j}")
 
 
-@pytest.mark.parametrize("kind", ["fp8", "int8"])
-def test_zero_v_rows_at_the_end_under_alibi(api, kind):
-    hq, hk, dim, n = 8, 2, 128, 700
+@pytest.mark.parametrize("kind,hq,hk,dim", CODES + STREAM)
+def test_zero_v_rows_at_the_end_under_alibi(api, kind, hq, hk, dim):
+    n = 700
     parts = cache_of(n, hk, dim, kind, 7)
     parts[2][-300:], parts[3][-300:] = 0.0, 0.0
     check(api, query(hq, dim, torch.bfloat16), parts, kind, alibi=True, what=kind)
@@ -94,3 +96,31 @@ def test_all_v_rows_are_zeros(api):
         q = query(8, 128, torch.float16)
         check(api, q, parts, kind, what=kind)
         assert (run(api, q, parts, kind)[0] == 0).all()
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("kind,hq,hk,dim", STREAM)
+def test_one_key_far_ahead_of_many(api, kind, hq, hk, dim, dt):
+    """The leading key's V row is zero in half of the dims: there the output is what the many small weights come to, and
+    none of them may be lost, while the leading weight itself is an ordinary one."""
+    q = query(hq, dim, DTYPES[dt])
+    for n, nats, j in ((20000, 16.0, 0), (20000, 14.0, 19999), (6000, 17.0, 3000)):
+        parts = cache_of(n, hk, dim, kind, 9)
+        raise_key(q, parts[0], parts[1], j, nats)
+        parts[2][j, :, ::2] = 0.0
+        check(api, q, parts, kind, what=f"{kind} {hq}/{hk} {dim} {dt} {nats} nats, key {j} of {n}")
+
+
+@pytest.mark.parametrize("kind,hq,hk,dim", STREAM)
+def test_v_rows_of_any_size(api, kind, hq, hk, dim):
+    """Stretches of a sequence whose V scales are 2^100 apart, next to scores that rise, fall or stay."""
+    n = 1000
+    q = query(hq, dim, torch.bfloat16)
+    for sizes in ((0, -100, 0), (-100, 0, -100, 100), (100, 0, -100), (-60, -100, 40, 100, 0), (0, 0, -100), (60, -60, 60)):
+        for slope in (0.0, 2.0, -2.0):
+            parts = cache_of(n, hk, dim, kind, 10)
+            at = torch.arange(n, device=DEV) * len(sizes) // n
+            parts[3] *= torch.exp2(torch.tensor(sizes, device=DEV, dtype=torch.float32)[at]).unsqueeze(-1)
+            parts[0][:] = parts[0][:1]  # equal scores, times the ramp
+            parts[1][:] = parts[1][:1] * torch.exp2(slope * torch.linspace(-2, 2, n, device=DEV)).unsqueeze(-1) * 8
+            check(api, q, parts, kind, what=f"{kind} {hq}/{hk} {dim} {sizes} slope {slope}")
