@@ -7,10 +7,12 @@
 // Here the work of the CUDA cores is per KEY and head, not per element:
 //     S^T[128 keys x N] = K[128 x D] . Qp^T,     O^T[D x N] += V^T[D x 128 keys] . Pp^T
 // K and V (e4m3, or s8) are the A operands of tcgen05.mma, the other side is 8 bits wide too and comes in PIECES, columns of
-// their own: q and the weights w_j = p_j vs_j as hi, mid and lo parts that add up to
-//   int8:  23-bit (q, signed) and 23-bit (w) fixed point, digits of 2^16, 2^8 and 1; kind::i8 sums them exactly in int32
-//   e4m3:  three e4m3 numbers, each the rounding of what the ones before it left over, times 16 (kind::f8f6f4)
-// so that q is exact to 2^-22 of its head's largest element and a weight to 2^-12 of itself or 2^-23 of the largest one.
+// their own: q as three parts and the weights w_j = p_j vs_j as four that add up to
+//   int8:  23-bit (q, signed) and 31-bit (w) fixed point, eight bits a digit; kind::i8 sums them exactly in int32
+//   e4m3:  e4m3 numbers, each the rounding of what the ones before it left over, times 16 (kind::f8f6f4)
+// so that q is exact to 2^-22 of its head's largest element and a weight to 2^-31 of the largest one (int8), or to 2^-11 of
+// itself and 2^-29 of the largest one (e4m3).  (With three parts of a weight, 2^-23 and 2^-25, the many small weights next to a
+// key that leads by 16 nats were lost from o while the denominator had them.)
 //
 // A CTA takes one KV head and an equal span of the batch's keys (StreamParams), three CTAs an SM.  Warps: four softmax
 // warps, a thread per key of a tile (the sum over a row's keys needs no order among threads until the end), one producer
@@ -33,7 +35,7 @@ constexpr int kKeys = 128;              // of a tile
 constexpr int kRowBytes = 128;          // of a staged row: D codes, or 96 and zeros
 constexpr int kTileBytes = kKeys * kRowBytes;
 constexpr int kHeads = 4;
-constexpr int kN = 16;                  // columns: piece * kHeads + head, and four that nobody reads
+constexpr int kN = 16;                  // columns: piece * kHeads + head; of the scores' last four nobody reads
 constexpr int kCtas = 3;                // per SM
 constexpr int kSoftmaxThreads = 128;
 constexpr int kThreads = 256;           // (the last warp only fills up)
@@ -64,7 +66,7 @@ struct HeadState {
     float factor;     // of a score: softmax scale * log2(e), q's unit
     float slope;      // ALiBi
     float m, mw;      // reference maxima of the scores and of the weights, log2
-    float g;          // 2^(m - mw)
+    float g;          // 2^((m - mw) / 2): one half goes to the probability, one to the V scale, so that both stay inside fp32
     float pad[3];
 };
 
@@ -286,8 +288,8 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
         // q's largest element is brought to 2^22 (int: |pieces| <= 127) or 2^8 (e4m3)
         constexpr int kQTop = kInt ? 22 : 8;
-        // weights: 2^22 (int) or 2^7 (e4m3) at the reference, twice that at most
-        constexpr float kWUnit = kInt ? 4194304.0f : 128.0f;
+        // weights: 2^30 (int) or 2^7 (e4m3) at the reference, twice that at most
+        constexpr float kWUnit = kInt ? 1073741824.0f : 128.0f;
         int t = 0;
         for (; more; ++x.b, more = x.load(p, plan, span)) {
             // ---- q in pieces: a warp per head, four elements a lane ----
@@ -377,7 +379,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
             int row = row_of(0), row_next = row_of(1);
             float ks = row >= 0 ? p.k_scale[(long long)row * p.head_k + head_k] : 0.0f;
             float vs = row >= 0 ? p.v_scale[(long long)row * p.head_k + head_k] : 0.0f;
-            // What the tensor core holds, in fp32 and in units of 2^mw: three pieces a head.
+            // What the tensor core holds, in fp32 and in units of 2^mw: four pieces a head.
             auto accumulated = [&](float (&sum)[kHeads]) {
                 uint32_t r[kN];
                 tmem_ld16(lanes + kColO, r);
@@ -385,10 +387,13 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
 #pragma unroll
                 for (int h = 0; h < kHeads; ++h) {
                     if (kInt) {
-                        sum[h] = fmaf((float)(int)r[h], 65536.0f, fmaf((float)(int)r[kHeads + h], 256.0f, (float)(int)r[2 * kHeads + h])) *
-                                 (1.0f / kWUnit);
+                        const float hi = fmaf((float)(int)r[h], 256.0f, (float)(int)r[kHeads + h]);
+                        const float lo = fmaf((float)(int)r[2 * kHeads + h], 256.0f, (float)(int)r[3 * kHeads + h]);
+                        sum[h] = fmaf(hi, 65536.0f, lo) * (1.0f / kWUnit);
                     } else {
-                        sum[h] = fmaf(__uint_as_float(r[2 * kHeads + h]), 1.0f / 256, fmaf(__uint_as_float(r[kHeads + h]), 1.0f / 16, __uint_as_float(r[h]))) / kWUnit;
+                        const float hi = fmaf(__uint_as_float(r[kHeads + h]), 1.0f / 16, __uint_as_float(r[h]));
+                        const float lo = fmaf(__uint_as_float(r[3 * kHeads + h]), 1.0f / 16, __uint_as_float(r[2 * kHeads + h]));
+                        sum[h] = fmaf(lo, 1.0f / 256, hi) * (1.0f / kWUnit);
                     }
                 }
             };
@@ -475,7 +480,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                         c = fmaxf(c, a - kWeightReach);
                         hs[tid].m = a;
                         hs[tid].mw = c;
-                        hs[tid].g = exp2f(a - c);
+                        hs[tid].g = exp2f(0.5f * (a - c));
                     }
                     if (since > 0) {  // the last contraction has finished: take over what it has
                         ok &= (bool)__all_sync(0xffffffffu, mbar_wait(&p_empty[(t - 1) & 1], (uint32_t)((t - 1) >> 1) & 1u, abort_flag));
@@ -495,7 +500,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                 // ---- weights, in pieces, as the other contraction's operand ----
                 if (t >= 2) ok &= (bool)__all_sync(0xffffffffu, mbar_wait(&p_empty[sb], ((uint32_t)(t >> 1) & 1u) ^ 1u, abort_flag));
                 uint8_t *pt = smem + kOffP + sb * kN * kRowBytes;
-                const float scaled_vs = valid ? my_vs * kWUnit : 0.0f;
+                const float w_vs = valid ? my_vs : 0.0f;
 #pragma unroll
                 for (int h = 0; h < kHeads; h += 2) {
                     float w[2];
@@ -503,24 +508,25 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                     for (int e = 0; e < 2; ++e) {
                         const float pr = exp2f(s[h + e] - hs[h + e].m);
                         l[h + e] += pr;
-                        w[e] = (pr * hs[h + e].g) * scaled_vs;  // (in this order: vs g alone may be past fp32)
+                        w[e] = (pr * hs[h + e].g) * (w_vs * (hs[h + e].g * kWUnit));
                     }
                     if (kInt) {
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const uint32_t bits = __float_as_uint(fminf(w[e], 8388607.0f) + 8388608.0f);  // 23 bits of it
-                            pt[swizzled(h + e, tid)] = (uint8_t)(bits >> 16);
-                            pt[swizzled(kHeads + h + e, tid)] = (uint8_t)(bits >> 8);
-                            pt[swizzled(2 * kHeads + h + e, tid)] = (uint8_t)bits;
+                            const uint32_t bits = __float2uint_rn(w[e]);
+                            pt[swizzled(h + e, tid)] = (uint8_t)(bits >> 24);
+                            pt[swizzled(kHeads + h + e, tid)] = (uint8_t)(bits >> 16);
+                            pt[swizzled(2 * kHeads + h + e, tid)] = (uint8_t)(bits >> 8);
+                            pt[swizzled(3 * kHeads + h + e, tid)] = (uint8_t)bits;
                         }
                     } else {
                         __half2 v = __floats2half2_rn(w[0], w[1]);
 #pragma unroll
-                        for (int k = 0; k < 3; ++k) {
+                        for (int k = 0; k < 4; ++k) {
                             const uint32_t c = e4m3x2(v);
                             pt[swizzled(k * kHeads + h, tid)] = (uint8_t)c;
                             pt[swizzled(k * kHeads + h + 1, tid)] = (uint8_t)(c >> 8);
-                            if (k < 2) v = __hmul2(__hsub2(v, from_e4m3x2(c)), __half2half2(__float2half_rn(16.0f)));
+                            if (k < 3) v = __hmul2(__hsub2(v, from_e4m3x2(c)), __half2half2(__float2half_rn(16.0f)));
                         }
                     }
                 }
@@ -567,7 +573,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                 if (h >= heads) break;
                 const float sum = red[h].x + red[kHeads + h].x + red[2 * kHeads + h].x + red[3 * kHeads + h].x;
                 // o is in units of 2^mw, the sum in units of 2^m
-                const float v = (sum > 0.0f ? o[h] * (1.0f / sum) * (1.0f / hs[h].g) : (sum == 0.0f ? 0.0f : sum)) + odd;
+                const float v = (sum > 0.0f ? o[h] * (1.0f / sum) * (1.0f / hs[h].g) * (1.0f / hs[h].g) : (sum == 0.0f ? 0.0f : sum)) + odd;
                 const long long out = (long long)x.b * p.head_q + head0 + h;
                 const long long piece = (span * 2 + (x.begin == 0 ? 1 : 0)) * p.head_q + head0 + h;
                 const float lse = sum == 0.0f ? -INFINITY : (hs[h].m + log2f(sum)) * kLn2;

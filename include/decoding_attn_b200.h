@@ -246,7 +246,8 @@ typedef struct da_quant_decode_args {
 
 /* o = softmax(scale * q . (k k_scale)^T + alibi) . (v v_scale) for one query token per sequence.  The work is cut by
  * keys on the device, so no length hint is taken.  Codes enter exactly; the softmax weights (times the V scales) are rounded
- * to 11 bits or, where they are small, to 2^-22 of the largest one; sums are fp32 or exact integers.  Scales are not negative.
+ * to 11 bits or, where they are small, to 2^-29 of the head's largest one (below 2^-120 they count as zero); sums are fp32 or
+ * exact integers.  Scales are not negative.
  * A zero-length sequence, or one whose keys are all masked, gives a zero row and
  * LSE = -inf.  The workspace needs no clearing; calls that may overlap need one each.  Graph-capturable. */
 int da_quant_decode_fwd(const da_quant_decode_args_t *args);

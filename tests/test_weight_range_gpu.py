@@ -99,7 +99,7 @@ def test_all_v_rows_are_zeros(api):
 
 
 @pytest.mark.parametrize("dt", ["fp16", "bf16"])
-@pytest.mark.parametrize("kind,hq,hk,dim", STREAM)
+@pytest.mark.parametrize("kind,hq,hk,dim", CODES + STREAM)
 def test_one_key_far_ahead_of_many(api, kind, hq, hk, dim, dt):
     """The leading key's V row is zero in half of the dims: there the output is what the many small weights come to, and
     none of them may be lost, while the leading weight itself is an ordinary one."""
@@ -111,12 +111,12 @@ def test_one_key_far_ahead_of_many(api, kind, hq, hk, dim, dt):
         check(api, q, parts, kind, what=f"{kind} {hq}/{hk} {dim} {dt} {nats} nats, key {j} of {n}")
 
 
-@pytest.mark.parametrize("kind,hq,hk,dim", STREAM)
+@pytest.mark.parametrize("kind,hq,hk,dim", CODES + STREAM)
 def test_v_rows_of_any_size(api, kind, hq, hk, dim):
     """Stretches of a sequence whose V scales are 2^100 apart, next to scores that rise, fall or stay."""
     n = 1000
     q = query(hq, dim, torch.bfloat16)
-    for sizes in ((0, -100, 0), (-100, 0, -100, 100), (100, 0, -100), (-60, -100, 40, 100, 0), (0, 0, -100), (60, -60, 60)):
+    for sizes in ((0, -100, 0), (-100, 0, -100, 100), (100, 0, -100), (-60, -100, 40, 100, 0), (0, 0, -100), (60, -60, 60), (0, 112, -100), (112,), (-100,)):
         for slope in (0.0, 2.0, -2.0):
             parts = cache_of(n, hk, dim, kind, 10)
             at = torch.arange(n, device=DEV) * len(sizes) // n
@@ -124,3 +124,21 @@ def test_v_rows_of_any_size(api, kind, hq, hk, dim):
             parts[0][:] = parts[0][:1]  # equal scores, times the ramp
             parts[1][:] = parts[1][:1] * torch.exp2(slope * torch.linspace(-2, 2, n, device=DEV)).unsqueeze(-1) * 8
             check(api, q, parts, kind, what=f"{kind} {hq}/{hk} {dim} {sizes} slope {slope}")
+
+
+@pytest.mark.parametrize("kind,dim", [("int8", 128), ("fp8", 128), ("int8", 96), ("int4", 64), ("fp8", 64)])
+def test_one_key_far_ahead_in_a_block_with_many(api, kind, dim):
+    """With as many heads as this a block has thousands of keys, which share its references with the leading one."""
+    hk, n = 128, 40000
+    q = query(hk, dim, torch.float16)
+    parts = cache_of(n, hk, dim, kind, 11)
+    for j in (0, 20011):
+        raise_key(q, parts[0], parts[1], j, 16.0)
+        parts[2][j, :, ::2] = 0.0
+    few = slice(0, hk, 41)
+    o, lse = run(api, q, parts, kind)
+    found = weight_bounds.attend(q[few], parts[0][:, few], parts[1][:, few].float(), parts[2][:, few], parts[3][:, few].float())
+    tol, tol_lse = weight_bounds.bounds(found, n, 11, o.dtype)
+    assert ((lse[0, few].double() - found["lse"]).abs() <= tol_lse).all()
+    over = (o[0, few].double() - found["o"]).abs() / tol
+    assert (over <= 1.0).all(), f"{kind} {dim}: {over.max().item():.3g} of the bound"
