@@ -37,7 +37,12 @@ constexpr int kBlockBytes = 128 * 128;  // [128 rows or keys][64 columns]
 constexpr int kSlots = 5;
 constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 384;  // (warps 10 and 11 only fill up the third warpgroup)
-constexpr float kRescaleThreshold = 8.0f;
+constexpr float kRescaleThreshold = 8.0f;  // log2 of what a score may exceed the maximum by that the reference stands for
+// The softmax weights are rounded to the type of V, which the instruction wants on both sides.  fp16: the reference is 2^-7
+// of the largest weight, so that fp16's subnormal numbers begin at 2^-21 of it and not at 2^-14; the weights then reach
+// 2^15.  (bf16 has fp32's range.)
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 
 template <int N, bool kMore>
 __device__ __forceinline__ void set_max_registers() {
@@ -324,12 +329,12 @@ da_prefix_kernel(const PrefixParams p, const __grid_constant__ CUtensorMap tm_q,
                     for (int j = 1; j < 32; ++j) top[c] = fmaxf(top[c], __uint_as_float(s[c][j]));
                 }
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
-                const bool raise = valid && mx > m + kRescaleThreshold;
+                const bool raise = valid && mx > m + (kRescaleThreshold + kLift<T>);
                 if (__any_sync(0xffffffffu, raise)) {
                     float shrink = 1.0f;
                     if (raise) {
-                        shrink = exp2f(m - mx);  // 0 on the first tile
-                        m = mx;
+                        shrink = exp2f(m - (mx - kLift<T>));  // 0 on the first tile
+                        m = mx - kLift<T>;
                         sum *= shrink;
                     }
                     if (i > 0) {  // the accumulator is idle once the last P.V of this stream has finished

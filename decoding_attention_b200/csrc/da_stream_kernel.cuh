@@ -26,8 +26,9 @@
 // exact, but for elements of a bf16 head below 2^-14 of its largest, which keep 2^-25 of that.  The weights w_j = p_j vs_j
 // are rounded to fp16 in units of their own, a power of two per head that is kept like the reference maximum: the largest
 // weight so far comes to 2^7..2^15, so that a weight is off by half a step, 2^-11 of itself, or by 2^-32 of the largest.
-// (The units follow the weights and not the probabilities: a key that leads by far may have a V row of zeros.)  Between q
-// and o these are the only roundings to fewer bits; sums, maxima and outputs are fp32.
+// (The units follow the weights and not the probabilities: a key that leads by far may have a V row of zeros.)  16-bit
+// caches: the weights are the probabilities, rounded to the cache's type, which V has and the instruction wants on both
+// sides.  Between q and o these are the only roundings to fewer bits; sums, maxima and outputs are fp32.
 //
 // Work split.  Lengths live on the device, so the CTAs cut the concatenated keys of the whole batch into equal spans
 // (StreamParams): any mix of lengths keeps all SMs busy to the end, without a sort or a guess of the longest sequence.
@@ -293,6 +294,9 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
     using C = StreamCfg<KIND, D, NT>;
     constexpr int TK = C::TK, RB = C::RB, STAGES = C::STAGES, MT = TK / 16;
     constexpr bool kBf16 = KIND == 4;
+    // fp16 weights (16-bit caches): the reference is 2^-7 of the largest, so that fp16's subnormal numbers begin at 2^-21 of
+    // it and not at 2^-14; the weights then reach 2^15.  (bf16 has fp32's range.)
+    constexpr float kLift = KIND == 0 ? 7.0f : 0.0f;
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r = lane >> 2, c = lane & 3;
@@ -621,7 +625,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                     float top = s[0][n][e];
 #pragma unroll
                     for (int t = 0; t < MT; ++t) top = fmaxf(top, fmaxf(s[t][n][e], s[t][n][2 + e]));
-                    raise |= top > m[n][e] + 8.0f;
+                    raise |= top > m[n][e] + (8.0f + kLift);
                 }
             // New units for the weights too, where V rows far larger than those before would leave fp32 in the old ones.
             float v_top = 0.0f;
@@ -641,7 +645,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                     for (int e = 0; e < 2; ++e) {
                         float top = m[n][e];
 #pragma unroll
-                        for (int t = 0; t < MT; ++t) top = fmaxf(top, fmaxf(s[t][n][e], s[t][n][2 + e]));
+                        for (int t = 0; t < MT; ++t) top = fmaxf(top, fmaxf(s[t][n][e], s[t][n][2 + e]) - kLift);
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                         float shrink = exp2_fast(m[n][e] - top);
