@@ -38,6 +38,8 @@
 // tiles (cp.async, zero fill for rows that are masked or that no page holds), filled across the ends of sequences.
 #pragma once
 
+#include <cfloat>
+
 #include "da_internal.h"
 #include "da_stream.h"
 
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) m[n][e] = -1e30f, l[n][e] = 0.0f, f[n][e] = 1.0f;
+            for (int e = 0; e < 2; ++e) m[n][e] = -FLT_MAX, l[n][e] = 0.0f, f[n][e] = 1.0f;
 #pragma unroll
         for (int t = 0; t < C::MTILES; ++t)
 #pragma unroll

@@ -55,3 +55,20 @@ def test_one_key_far_ahead_in_a_block_with_many(api, dtype, bits):
     for dim in (64, 128):
         lead_and_check(api, dtype, bits, dim, 64, 8, 512, 4000, 1, [(0, 0), (0, 2500)], 16.3)
         lead_and_check(api, dtype, bits, dim, 8, 8, 300, 100, 3000, [(1, 0), (1, 1777)], 16.3)
+
+
+@pytest.mark.parametrize("prefix,own", [(0, 40), (150, 0), (150, 40)])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_scores_near_the_end_of_fp32(api, sign, prefix, own):
+    """Keys that are all alike, with scores of +-2^122: the output is the mean of V."""
+    dim, hq, hk = 128, 8, 2
+    g = torch.Generator(device=DEV).manual_seed(4)
+    k = [torch.full((n, hk, dim), 2.0 ** 62, device=DEV, dtype=torch.bfloat16) for n in (prefix, own)]
+    v = [torch.randn(n, hk, dim, device=DEV, generator=g).to(torch.bfloat16) for n in (prefix, own)]
+    q = torch.full((1, hq, dim), sign * 2.0 ** 60 / dim, device=DEV, dtype=torch.bfloat16)
+    cu = torch.tensor([0, own], dtype=torch.int32, device=DEV)
+    o, lse = api.shared_prefix_fwd(q, k[0], v[0], k[1], v[1], cu, softmax_scale=1.0, return_lse=True)
+    ones = torch.ones(prefix + own, hk, device=DEV)
+    found = weight_bounds.attend(q[0], torch.cat(k), ones, torch.cat(v), ones, softmax_scale=1.0)
+    tol, tol_lse = weight_bounds.bounds(found, prefix + own, 8, q.dtype)
+    assert ((lse[0].double() - found["lse"]).abs() <= tol_lse).all() and ((o[0].double() - found["o"]).abs() <= tol).all()

@@ -142,3 +142,14 @@ def test_one_key_far_ahead_in_a_block_with_many(api, kind, dim):
     assert ((lse[0, few].double() - found["lse"]).abs() <= tol_lse).all()
     over = (o[0, few].double() - found["o"]).abs() / tol
     assert (over <= 1.0).all(), f"{kind} {dim}: {over.max().item():.3g} of the bound"
+
+
+@pytest.mark.parametrize("kind,hq,hk,dim", CODES + STREAM)
+def test_scores_near_the_end_of_fp32(api, kind, hq, hk, dim):
+    """Keys that are all alike, with scores of +-2^122: the output is the mean of V."""
+    for sign in (-1.0, 1.0):
+        for n in (5, 300):
+            parts = cache_of(n, hk, dim, kind, 12)
+            parts[0][:], parts[1][:] = 4.0, 2.0 ** 60
+            q = torch.full((hq, dim), sign * 2.0 ** 60 / dim, device=DEV).to(torch.bfloat16)
+            check(api, q, parts, kind, softmax_scale=1.0, what=f"{kind} {sign} {n}")
