@@ -508,9 +508,10 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     // 2^-e and 2^e of the largest element; zeros, infinities and NaN stay as they are
                     const int ex = (int)(__float_as_uint(top) >> 23);
-                    if (ex > 1 && ex < 253) {
-                        up = __uint_as_float((uint32_t)(254 - ex) << 23);
-                        f = p.scale_log2 * __uint_as_float((uint32_t)ex << 23);
+                    if (ex > 1 && ex < 255) {
+                        const int e = min(ex, 253);  // (2^-e is a normal number then)
+                        up = __uint_as_float((uint32_t)(254 - e) << 23);
+                        f = p.scale_log2 * __uint_as_float((uint32_t)e << 23);
                     }
                 }
 #pragma unroll

@@ -153,3 +153,12 @@ def test_scores_near_the_end_of_fp32(api, kind, hq, hk, dim):
             parts[0][:], parts[1][:] = 4.0, 2.0 ** 60
             q = torch.full((hq, dim), sign * 2.0 ** 60 / dim, device=DEV).to(torch.bfloat16)
             check(api, q, parts, kind, softmax_scale=1.0, what=f"{kind} {sign} {n}")
+
+
+@pytest.mark.parametrize("kind,hq,hk,dim", CODES + STREAM)
+def test_largest_and_smallest_queries(api, kind, hq, hk, dim):
+    for at, scale in ((127, 2.0 ** -30), (126, 2.0 ** -30), (-90, 2.0 ** 80)):
+        parts = cache_of(200, hk, dim, kind, 13)
+        parts[1] *= 2.0 ** (-95 if at > 0 else 5)
+        q = (query(hq, dim, torch.float32).clamp(-1.9, 1.9) * 2.0 ** (at - 64) * 2.0 ** 64).to(torch.bfloat16)
+        check(api, q, parts, kind, softmax_scale=scale, what=f"{kind} 2^{at}")
