@@ -1,5 +1,6 @@
 // C ABI of the operators around a quantised cache -- writing rows, reading them back, decode attention over them -- and
 // of decode attention behind a shared prefix.
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -24,16 +25,16 @@ int failf(int code, const char *fmt, ...) {
 }
 
 int sm_count(int *out) {
-    static int known[64];  // 0: not asked yet (every thread would store the same value)
+    static std::atomic<int> known[64];  // 0: not asked yet
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && dev < 64 && known[dev] > 0) {
-        *out = known[dev];
-        return DA_OK;
+    if (e == cudaSuccess && dev < 64) {
+        *out = known[dev].load(std::memory_order_relaxed);
+        if (*out > 0) return DA_OK;
     }
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return failf(DA_ERR_CUDA, "device query: %s", cudaGetErrorString(e));
-    if (dev < 64) known[dev] = *out;
+    if (dev < 64) known[dev].store(*out, std::memory_order_relaxed);
     return DA_OK;
 }
 
