@@ -47,17 +47,17 @@ StreamShape stream_shape(int dim, int kind, int group) {
     }
 }
 
-cudaError_t launch_stream(int dim, int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap) {
+namespace {
+cudaError_t launch_stream(int dim, int kind, bool bf16, const StreamParams &p, cudaStream_t s) {
     switch (dim) {
-        case 64: return launch_stream_d64(kind, bf16, p, s, overlap);
-        case 96: return launch_stream_d96(kind, bf16, p, s, overlap);
-        case 128: return launch_stream_d128(kind, bf16, p, s, overlap);
-        case 256: return launch_stream_d256(kind, bf16, p, s, overlap);
+        case 64: return launch_stream_d64(kind, bf16, p, s);
+        case 96: return launch_stream_d96(kind, bf16, p, s);
+        case 128: return launch_stream_d128(kind, bf16, p, s);
+        case 256: return launch_stream_d256(kind, bf16, p, s);
         default: return cudaErrorInvalidValue;
     }
 }
 
-namespace {
 // Whether the tensor-core kernel for codes takes the call: 8-bit codes of head dims and groups that it has, in pages that a
 // TMA box can fetch, and pieces that are worth its 128-key tiles.  With no more (sequence, KV head) pairs than CTA slots it
 // is the faster one at any length (one sequence of 1 500 keys, 8 KV heads: 8.7 us against 10.5); with more, a CTA works
@@ -92,7 +92,7 @@ int run_stream(int dim, int kind, bool bf16, const StreamParams &p, cudaStream_t
         if (rc != DA_OK) return rc;
         e = launch_codes(dim, kind, p, status, tm_k, tm_v, s);
     } else {
-        e = launch_stream(dim, kind, bf16, p, s, true);
+        e = launch_stream(dim, kind, bf16, p, s);
     }
     if (e != cudaSuccess) return failf(DA_ERR_CUDA, "decode kernel launch: %s", cudaGetErrorString(e));
     return DA_OK;

@@ -468,7 +468,6 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                         }
                         l[h] *= exp2f(m0 - a);
                         shrink[h] = exp2f(mw0 - fmaxf(c, a - kWeightReach));
-                        s[h] = valid ? s[h] : -INFINITY;
                     }
                     named_bar_sync(2, kSoftmaxThreads);
                     if (tid < kHeads) {

@@ -54,10 +54,10 @@ StreamShape stream_shape_d64(int kind, int group);
 StreamShape stream_shape_d96(int kind, int group);
 StreamShape stream_shape_d128(int kind, int group);
 StreamShape stream_shape_d256(int kind, int group);
-cudaError_t launch_stream_d64(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
-cudaError_t launch_stream_d96(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
-cudaError_t launch_stream_d128(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
-cudaError_t launch_stream_d256(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
+cudaError_t launch_stream_d64(int kind, bool bf16, const StreamParams &p, cudaStream_t s);
+cudaError_t launch_stream_d96(int kind, bool bf16, const StreamParams &p, cudaStream_t s);
+cudaError_t launch_stream_d128(int kind, bool bf16, const StreamParams &p, cudaStream_t s);
+cudaError_t launch_stream_d256(int kind, bool bf16, const StreamParams &p, cudaStream_t s);
 
 // The tensor-core kernel for 8-bit codes (da_codes_sm100.cu), head dims 96 and 128, groups of at most codes_heads() query
 // heads: p.spans spans, cuts at multiples of 128 keys, pages of 16 keys or more.  kind: 1 FP8 e4m3, 2 int8.  tm_k, tm_v:

@@ -2,8 +2,8 @@
 #include "da_stream_kernel.cuh"
 
 namespace da {
-cudaError_t launch_stream_d128(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap) {
-    return launch_stream_dim<128>(kind, bf16, p, s, overlap);
+cudaError_t launch_stream_d128(int kind, bool bf16, const StreamParams &p, cudaStream_t s) {
+    return launch_stream_dim<128>(kind, bf16, p, s);
 }
 StreamShape stream_shape_d128(int kind, int group) { return stream_shape_dim<128>(kind, group); }
 }  // namespace da

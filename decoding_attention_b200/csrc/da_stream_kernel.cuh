@@ -872,7 +872,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
 }
 
 template <int KIND, int D, int NT>
-cudaError_t launch_stream_variant(const StreamParams &p, cudaStream_t s, bool overlap) {
+cudaError_t launch_stream_variant(const StreamParams &p, cudaStream_t s) {
     using C = StreamCfg<KIND, D, NT>;
     auto kernel = da_stream_kernel<KIND, D, NT>;
     static thread_local uint64_t ready = 0;  // devices on which this thread has raised the kernel's shared-memory limit
@@ -887,7 +887,7 @@ cudaError_t launch_stream_variant(const StreamParams &p, cudaStream_t s, bool ov
     const int streams = p.head_k * p.chunks;
     const dim3 grid(p.spans, (streams + p.head_warps - 1) / p.head_warps);
     count_launch();
-    return launch_kernel(kernel, grid, kStreamWarps * 32, C::kSmemBytes, s, overlap, p);
+    return launch_kernel(kernel, grid, kStreamWarps * 32, C::kSmemBytes, s, true, p);
 }
 
 // Query heads of a warp: 16 where the accumulators of two column tiles fit, 8 otherwise.
@@ -897,20 +897,20 @@ constexpr int stream_nt(int group) {
 }
 
 template <int D>
-cudaError_t launch_stream_dim(int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap) {
+cudaError_t launch_stream_dim(int kind, bool bf16, const StreamParams &p, cudaStream_t s) {
     if constexpr (D <= 128) {
         if (stream_nt<D>(p.group) == 2) {
-            if (kind == 1) return launch_stream_variant<1, D, 2>(p, s, overlap);
-            if (kind == 2) return launch_stream_variant<2, D, 2>(p, s, overlap);
-            if (kind == 3) return launch_stream_variant<3, D, 2>(p, s, overlap);
-            return bf16 ? launch_stream_variant<4, D, 2>(p, s, overlap) : launch_stream_variant<0, D, 2>(p, s, overlap);
+            if (kind == 1) return launch_stream_variant<1, D, 2>(p, s);
+            if (kind == 2) return launch_stream_variant<2, D, 2>(p, s);
+            if (kind == 3) return launch_stream_variant<3, D, 2>(p, s);
+            return bf16 ? launch_stream_variant<4, D, 2>(p, s) : launch_stream_variant<0, D, 2>(p, s);
         }
     }
-    if (kind == 1) return launch_stream_variant<1, D, 1>(p, s, overlap);
-    if (kind == 2) return launch_stream_variant<2, D, 1>(p, s, overlap);
-    if (kind == 3) return launch_stream_variant<3, D, 1>(p, s, overlap);
+    if (kind == 1) return launch_stream_variant<1, D, 1>(p, s);
+    if (kind == 2) return launch_stream_variant<2, D, 1>(p, s);
+    if (kind == 3) return launch_stream_variant<3, D, 1>(p, s);
     if constexpr (D <= 128) {
-        return bf16 ? launch_stream_variant<4, D, 1>(p, s, overlap) : launch_stream_variant<0, D, 1>(p, s, overlap);
+        return bf16 ? launch_stream_variant<4, D, 1>(p, s) : launch_stream_variant<0, D, 1>(p, s);
     }
     return cudaErrorInvalidValue;
 }

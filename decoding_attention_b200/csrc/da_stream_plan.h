@@ -15,6 +15,5 @@ bool quantised_kind(int32_t kv_dtype);
 void plan_stream(int dim, int kind, int sms, StreamParams *p);
 size_t stream_piece_bytes(const StreamParams &p, int dim);  // of part_o and part_lse together
 int run_stream(int dim, int kind, bool bf16, const StreamParams &p, cudaStream_t s);
-cudaError_t launch_stream(int dim, int kind, bool bf16, const StreamParams &p, cudaStream_t s, bool overlap);
 
 }  // namespace da
