@@ -120,21 +120,8 @@ __device__ __forceinline__ __half2 from_e4m3x2(uint32_t x) {
     return *reinterpret_cast<const __half2 *>(&r);
 }
 
-// The pieces of a span for one CTA, and its tiles in the order in which all roles take them.
-struct SpanWalk {
-    int b, start, len, begin, end;
-    __device__ __forceinline__ bool load(const StreamParams &p, const SpanPlan &s, long long span) {
-        for (; b < p.batch; ++b) {
-            start = p.cu_seq_k[b];
-            const long long at = axis_start(s, b, start);
-            if (at >= (span + 1) * s.units) return false;
-            len = sequence_keys(p, b, start);
-            if (len == 0) continue;
-            span_piece(s, span, at, len, begin, end);
-            if (begin < end) return true;
-        }
-        return false;
-    }
+// The pieces of a span, and their tiles in the order in which all roles take them.
+struct SpanWalk : PieceCursor {
     __device__ __forceinline__ int tiles() const { return (end - begin + kKeys - 1) / kKeys; }
     // ALiBi: back to front, the first tiles set the reference maxima
     __device__ __forceinline__ int key(const StreamParams &p, int i) const { return begin + (p.is_alibi ? tiles() - 1 - i : i) * kKeys; }
@@ -186,16 +173,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
     x.b = 0;
     bool more = span * plan.units < plan.total;
     if (more) {
-        // largest b that begins on the axis at or before the span
-        int lo = 0, n = p.batch;
-        while (n > 1) {
-            const int step = (n + 31) / 32, at = lane * step;
-            const unsigned hit = __ballot_sync(0xffffffffu, at < n && axis_start(plan, lo + at, p.cu_seq_k[lo + at]) <= span * plan.units);
-            const int off = hit ? (__popc(hit) - 1) * step : 0;
-            lo += off;
-            n = min(n - off, step);
-        }
-        x.b = lo;
+        x.b = find_sequence(plan, p.cu_seq_k, p.batch, span * plan.units, lane);
         more = x.load(p, plan, span);
     }
 

@@ -257,39 +257,6 @@ __device__ __forceinline__ void load_v_words(const uint8_t *tile, int row, int r
     if (RB & 16) w[i2] = *reinterpret_cast<const uint16_t *>(base + b2 + r * 2);
 }
 
-// The pieces of a span, in order.
-struct PieceCursor {
-    int b, start, len, begin, end;
-    __device__ __forceinline__ bool load(const StreamParams &p, const SpanPlan &s, long long span) {
-        // from sequence b on, the first one with keys in the span; false behind the last
-        for (; b < p.batch; ++b) {
-            start = p.cu_seq_k[b];
-            const long long at = axis_start(s, b, start);
-            if (at >= (span + 1) * s.units) return false;
-            len = sequence_keys(p, b, start);
-            if (len == 0) continue;
-            span_piece(s, span, at, len, begin, end);
-            if (begin < end) return true;
-        }
-        return false;
-    }
-};
-
-// Largest b in [0, batch) that begins on the axis at or before x, by the lanes of a warp together (0 if there is none).
-__device__ __forceinline__ int find_sequence(const SpanPlan &s, const int *cu, int batch, long long x, int lane) {
-    int lo = 0, n = batch;
-    while (n > 1) {
-        const int step = (n + 31) / 32;
-        const int at = lane * step;
-        const unsigned hit = __ballot_sync(0xffffffffu, at < n && axis_start(s, lo + at, cu[lo + at]) <= x);
-        const int count = __popc(hit);
-        const int off = count > 0 ? (count - 1) * step : 0;
-        lo += off;
-        n = n - off < step ? n - off : step;
-    }
-    return lo;
-}
-
 template <int KIND, int D, int NT>
 __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTwoCtas ? 2 : 1)
     da_stream_kernel(const StreamParams p) {
