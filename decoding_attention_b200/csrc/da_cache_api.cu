@@ -167,10 +167,12 @@ int check_rows_args(const da_kv_rows_args_t *a, bool write) {
 }
 
 int run_rows(const da_kv_rows_args_t *a, bool write) {
-    const int rc = check_rows_args(a, write);
+    int rc = check_rows_args(a, write);
     if (rc != DA_OK || a->tokens == 0) return rc;
     KvRowsParams p;
     memset(&p, 0, sizeof(p));
+    rc = sm_count(&p.sms);
+    if (rc != DA_OK) return rc;
     p.k = a->k;
     p.v = a->v;
     p.k_cache = a->k_cache;
@@ -424,6 +426,7 @@ int da_quant_decode_fwd(const da_quant_decode_args_t *a) {
     m.s.part_o = static_cast<float *>(a->workspace);
     m.s.part_lse = m.s.part_o + (size_t)m.s.spans * 2 * m.s.head_q * a->dim;
     m.dim = (int)a->dim;
+    m.sms = sms;
     m.o = a->o;
     m.lse = a->lse;
     cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
@@ -456,6 +459,7 @@ int da_prefix_decode_fwd(const da_prefix_decode_args_t *a) {
     m.s.part_o = parts + plan.parts + plan.own;
     m.s.part_lse = m.s.part_o + (size_t)m.s.spans * 2 * m.s.head_q * a->dim;
     m.dim = (int)a->dim;
+    m.sms = sms;
     m.o = a->o;
     m.lse = a->lse;
     cudaStream_t stream = static_cast<cudaStream_t>(a->stream);

@@ -266,7 +266,7 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
         HeadState *hs = reinterpret_cast<HeadState *>(smem + kOffHead);
         float2 *red = reinterpret_cast<float2 *>(smem + kOffRed);
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-        // q's largest element is brought to 2^22 (int: |pieces| <= 127) or 2^8 (e4m3)
+        // q's largest element is brought to 2^22 (int: digits of -128 to 127) or 2^8 (e4m3)
         constexpr int kQTop = kInt ? 22 : 8;
         // weights: 2^30 (int) or 2^7 (e4m3) at the reference, twice that at most
         constexpr float kWUnit = kInt ? 1073741824.0f : 128.0f;

@@ -15,8 +15,8 @@
 // A row belongs to L = D / 16 lanes that hold two pieces of 8 values (16-byte accesses on the 16-bit side, lanes side by
 // side); a thread has kRows rows in flight, since the slot, the row and (reading) the scale are a chain of two loads.
 // Writing is close to the issue limit, so what is done once a row is done for kRows rows at a time: the maxima of four
-// rows are joined by reduce-scatter (five shuffles for L = 8 where four xor reductions take twelve), after which every
-// lane has the maximum of one row and the two quotients are worked out once for all of them.
+// rows are joined by reduce-scatter (four shuffles for L = 8 where four xor reductions take twelve), after which every lane
+// has the maximum of one row, and the two quotients are worked out once for all of them (a shuffle a row hands them back).
 #include "da_internal.h"
 #include "da_kv_rows.h"
 
@@ -259,11 +259,11 @@ __global__ void __launch_bounds__(kThreads) da_kv_read_kernel(const KvRowsParams
     pdl_launch_dependents();
 }
 
-// Rows of a thread.  Few rows: one each, to spread them over the SMs.
+// Rows of a thread.  Few rows, fewer than four blocks an SM: one each, to spread them.
 template <typename T, int D, int KVQ>
 cudaError_t launch_rows(const KvRowsParams &p, bool write, cudaStream_t s) {
     constexpr uint32_t kBlockRows = kThreads / RowCfg<D>::kLanes;
-    const bool many = p.rows > 4u * kBlockRows * 148u;
+    const bool many = p.rows > 4u * kBlockRows * (uint32_t)p.sms;
     const uint32_t per_block = kBlockRows * (many ? 4u : 1u);
     const dim3 grid((p.rows + per_block - 1) / per_block, 2);
     count_launch();

@@ -72,7 +72,7 @@ struct StreamMergeParams {
     StreamParams s;
     const float *prefix_o, *prefix_lse;  // [max_parts][batch][head_q][dim], [max_parts][batch][head_q]; NULL: no prefix
     PrefixGrid prefix;
-    int dim;
+    int dim, sms;
     void *o;      // [batch, head_q, dim], rows s.o_row_stride apart
     float *lse;   // optional [batch, head_q]
 };

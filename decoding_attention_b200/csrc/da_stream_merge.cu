@@ -205,14 +205,15 @@ cudaError_t launch_merge_warps(const StreamMergeParams &p, int heads_per_warp, c
 template <int D>
 cudaError_t launch_merge_dim(const StreamMergeParams &p, cudaStream_t s) {
     // Parts of a row, as far as the host can tell: those of the prefix and the sequence's share of the spans.  A warp for
-    // every four of them, if the blocks then still fit the SMs at once (three each).  Otherwise a warp a row, and above 740
-    // blocks (five an SM) two rows a warp, which share the search for their parts.
+    // every four of them, if the blocks then still fit the SMs at once (three each; twice that for two warps and many parts).
+    // Otherwise a warp a row, and above five blocks an SM two rows a warp, which share the search for their parts.
     const int parts = (p.prefix_o ? p.prefix.max_parts : 0) + 1 + p.s.spans / p.s.batch;
     auto blocks = [&](int warps) { return (long long)p.s.batch * ((p.s.head_q * warps + 7) / 8); };
-    if (parts > 16 && blocks(8) <= 444) return launch_merge_warps<D, 8>(p, 1, s);
-    if (parts > 8 && blocks(4) <= 444) return launch_merge_warps<D, 4>(p, 1, s);
-    if (parts > 4 && blocks(2) <= (parts > 8 ? 888 : 444)) return launch_merge_warps<D, 2>(p, 1, s);
-    const bool many = blocks(1) > 740 && p.s.head_q > 8;
+    const int at_once = 3 * p.sms;
+    if (parts > 16 && blocks(8) <= at_once) return launch_merge_warps<D, 8>(p, 1, s);
+    if (parts > 8 && blocks(4) <= at_once) return launch_merge_warps<D, 4>(p, 1, s);
+    if (parts > 4 && blocks(2) <= (parts > 8 ? 2 * at_once : at_once)) return launch_merge_warps<D, 2>(p, 1, s);
+    const bool many = blocks(1) > 5 * p.sms && p.s.head_q > 8;
     return launch_merge_warps<D, 1>(p, many ? 2 : 1, s);
 }
 
