@@ -167,12 +167,10 @@ int check_rows_args(const da_kv_rows_args_t *a, bool write) {
 }
 
 int run_rows(const da_kv_rows_args_t *a, bool write) {
-    int rc = check_rows_args(a, write);
+    const int rc = check_rows_args(a, write);
     if (rc != DA_OK || a->tokens == 0) return rc;
     KvRowsParams p;
     memset(&p, 0, sizeof(p));
-    rc = sm_count(&p.sms);
-    if (rc != DA_OK) return rc;
     p.k = a->k;
     p.v = a->v;
     p.k_cache = a->k_cache;

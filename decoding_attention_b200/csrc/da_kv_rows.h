@@ -27,7 +27,6 @@ struct KvRowsParams {
     long long cache_rows;
     uint32_t rows;  // tokens * head_k
     int head_k;
-    int sms;        // of the device
     FastDiv by_heads;
 };
 // x_dtype: type of k and v (0 fp16, 1 bf16, 2 fp32, reading only); kvq: 1 FP8 e4m3, 2 int8, 3 int4.
