@@ -10,7 +10,7 @@
 // their own: q as three parts and the weights w_j = p_j vs_j as four that add up to
 //   int8:  23-bit (q, signed) and 31-bit (w) fixed point, eight bits a digit; kind::i8 sums them exactly in int32
 //   e4m3:  e4m3 numbers, each the rounding of what the ones before it left over, times 16 (kind::f8f6f4)
-// so that q is exact to 2^-22 of its head's largest element and a weight to 2^-31 of the largest one (int8), or to 2^-15 of
+// so that q is exact to 2^-22 of its head's largest element and a weight to 2^-31 of the largest one (int8), or to 2^-11 of
 // itself and 2^-29 of the largest one (e4m3).  (With three parts of a weight, 2^-23 and 2^-25, the many small weights next to a
 // key that leads by 16 nats were lost from o while the denominator had them.)
 //
@@ -112,11 +112,6 @@ __device__ __forceinline__ float int_to_float(uint32_t x) {  // |x| < 2^22
 __device__ __forceinline__ uint32_t e4m3x2(__half2 x) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t *>(&x)));
-    return r;
-}
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
     return r;
 }
 __device__ __forceinline__ __half2 from_e4m3x2(uint32_t x) {
@@ -504,16 +499,13 @@ da_codes_kernel(const StreamParams p, const int dim, int *status, const __grid_c
                             pt[swizzled(3 * kHeads + h + e, tid)] = (uint8_t)bits;
                         }
                     } else {
-                        // (the first part from fp32: what it leaves over has 11 bits of its own)
-                        uint32_t c = e4m3x2(w[0], w[1]);
-                        const float2 first = __half22float2(from_e4m3x2(c));
-                        __half2 v = __floats2half2_rn((w[0] - first.x) * 16.0f, (w[1] - first.y) * 16.0f);
+                        __half2 v = __floats2half2_rn(w[0], w[1]);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            if (k > 0) c = e4m3x2(v);
+                            const uint32_t c = e4m3x2(v);
                             pt[swizzled(k * kHeads + h, tid)] = (uint8_t)c;
                             pt[swizzled(k * kHeads + h + 1, tid)] = (uint8_t)(c >> 8);
-                            if (k > 0 && k < 3) v = __hmul2(__hsub2(v, from_e4m3x2(c)), __half2half2(__float2half_rn(16.0f)));
+                            if (k < 3) v = __hmul2(__hsub2(v, from_e4m3x2(c)), __half2half2(__float2half_rn(16.0f)));
                         }
                     }
                 }
