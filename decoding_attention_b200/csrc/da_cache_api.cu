@@ -60,9 +60,11 @@ cudaError_t launch_stream(int dim, int kind, bool bf16, const StreamParams &p, c
 
 // Whether the tensor-core kernel for codes takes the call: 8-bit codes of head dims and groups that it has, in pages that a
 // TMA box can fetch, and pieces that are worth its 128-key tiles.  With no more (sequence, KV head) pairs than CTA slots it
-// is the faster one at any length (one sequence of 1 500 keys, 8 KV heads: 8.7 us against 10.5); with more, a CTA works
-// through several short sequences, and a piece costs it more (1 000 sequences of 65-130 keys: 96 against 74 us; 256 of
-// 1 000-2 000: 150 against 175 us).  The lengths are on the device: what the cache holds a sequence is what there is to go by.
+// is the faster one at any length (one sequence of 1 500 int8 keys, 8 heads: 8.6 us against 11.1); with more, a CTA works
+// through several short sequences, and a piece costs it more (1 000 sequences of 65-130 keys, 32/8 heads: 93 us against 77 in
+// int8, 111 against 68 in FP8; 256 of 1 000-2 000: 139 against 173 and 145 against 148).  The lengths are on the device: what
+// the cache, or a row of the block table, holds a sequence is what there is to go by.  (A caller whose table is wider than
+// its sequences passes the columns in use.)
 bool on_codes_kernel(int dim, int kind, const StreamParams &p, int sms) {
     if ((kind != DA_KV_FP8_E4M3 && kind != DA_KV_INT8) || (dim != 96 && dim != 128) || p.group > codes_heads() || p.rows == 0) return false;
     if (p.block_table && p.page_shift < 4) return false;
@@ -121,8 +123,8 @@ void plan_stream(int dim, int kind, int sms, StreamParams *p) {
     p->spans = slots > blocks ? slots / blocks : 1;
     // A piece of a sequence costs a CTA about as long as 64 keys of a warp, however short it is (its queries, the joining of
     // its warps, its output), and a span is longer than that.  With few sequences the spans' shortest length matters more
-    // than their balance: half as much then.  (32 x 1 024-4 096 int4 keys, 32/2 heads: 24.7 us with a cost of 16, 23.5 with
-    // 32, 22.6 with 64; 4 x 500-2 000, 32/8 heads: 13.9, 13.2 and 15.4.)
+    // than their balance: half as much then.  (32 x 1 024-4 096 int4 keys, 32/2 heads: 25.0 us with a cost of 16, 24.0 with
+    // 32, 22.9 with 64; 4 x 500-2 000, 32/8 heads: 13.3, 12.5 and 14.3.)
     const int cost = p->batch >= 16 ? 64 : 32;
     p->piece_cost = cost * p->key_warps;
     p->min_span = (cost + 32) * p->key_warps;

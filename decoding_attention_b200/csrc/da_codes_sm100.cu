@@ -17,7 +17,7 @@
 // A CTA takes one KV head and an equal span of the batch's keys (StreamParams), three CTAs an SM.  Warps: four softmax
 // warps, a thread per key of a tile (the sum over a row's keys needs no order among threads until the end), one producer
 // (TMA), one issuer per contraction.  A tile is a chain -- scores, weights, the other contraction -- of about 2 us, which is
-// why one or two CTAs an SM are not enough (256 x 512-4096 FP8 keys, 8 KV heads: 250 us with two, 210 with three; 131 072
+// why one or two CTAs an SM are not enough (256 x 512-4096 FP8 keys, 8 KV heads: 250 us with two, 209 with three; 131 072
 // int8 keys x 32 heads: 213 and 186 us, 0.91 of the measured copy rate).  Reference maxima are common to the CTA and move
 // rarely: a tile asks once (one barrier with a vote) whether a score or a weight has outgrown its reference by a factor of
 // 2; if so, what the tensor core has accumulated moves to fp32 registers (a thread per dim), where it is rescaled.

@@ -10,7 +10,7 @@
 // whatever reads it sees NaN.
 //
 // Bound: HBM.  A row costs 2D bytes on the 16-bit side and D (or D / 2) + 4 on the other; nothing is read twice.  32 768
-// tokens x 8 KV heads of 128 into int8: 30 us, the copy rate; 131 072 tokens out of FP8: 124 us, the copy rate.  Single
+// tokens x 8 KV heads of 128 into int8: 32 us, the copy rate; 131 072 tokens out of FP8: 125 us, the copy rate.  Single
 // tokens: 1.3 us of a stream's time, a launch.
 // A row belongs to L = D / 16 lanes that hold two pieces of 8 values (16-byte accesses on the 16-bit side, lanes side by
 // side); a thread has kRows rows in flight, since the slot, the row and (reading) the scale are a chain of two loads.

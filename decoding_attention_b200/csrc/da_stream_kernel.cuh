@@ -13,14 +13,14 @@
 //     S^T[16 keys x 8 heads] = K[16 x D] . Q^T,      O^T[D x 8 heads] += V^T[D x 16] . P^T
 // The products' reduction index may be permuted freely, so a lane loads its elements with 16-byte accesses of
 // untransposed rows, and the transposition of V is two byte permutes per pair of keys.  S^T becomes P^T by one movmatrix
-// per 8 keys.  16 keys of 128 columns and eight heads take 421 (int4), 447 (e4m3) and 574 (int8) instructions, all told:
-// 4 x 65 536 keys with 64 over 8 heads come to 91 us (int4, HBM time 44), 105 (e4m3, 85) and 124 us (int8, 85).
+// per 8 keys.  16 keys of 128 columns and eight heads take 434 (int4), 462 (e4m3) and 589 (int8) instructions, all told:
+// 4 x 65 536 keys with 64 over 8 heads come to 89 us (int4, HBM time 44), 102 (e4m3, 85) and 118 us (int8, 85).
 //
 // For 8-bit codes and groups of up to four heads da_codes_sm100.cu, where the codes themselves are tensor-core operands, is
 // faster.  Tried for the rest and left out: the codes widened to fp16 in shared memory by warps of their own, once a key, as
 // tcgen05 operands (the chain of widening, scores, weights and the other contraction takes 3 000 cycles a tile with the one
 // CTA an SM that fits: 191 us for the int4 case above); and 32 heads a warp, so that a group of 32 is widened once instead
-// of twice (128 sequences of 2 048 int4 keys, 32 heads over one KV head: 51 us, 42 with two warps of 16 heads).
+// of twice (128 sequences of 2 048 int4 keys, 32 heads over one KV head: 51 us against 42 with two warps of 16 heads; 44 now).
 //
 // q is brought to fp16 with a power of two per head that makes its largest element 1..2, undone in the score's factor:
 // exact, but for elements of a bf16 head below 2^-14 of its largest, which keep 2^-25 of that.  The weights w_j = p_j vs_j

@@ -111,7 +111,8 @@ def quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, is_alibi=Fals
     q [batch, head_q, dim]; cu_seq_k int32 [batch + 1], cumulative lengths.  A packed cache holds key j of sequence b in
     row ``cu_seq_k[b] + j``; a paged one (4-D, page_size a power of two) in row ``j % page_size`` of page
     ``block_table[b, j // page_size]`` (int32).  Keys whose row or page lies outside the cache are masked.  No length hint
-    is needed: the work is divided on the device.  ``return_lse`` adds the fp32 natural-log LSE [batch, head_q].
+    is needed: the work is divided on the device.  (Which kernel takes 8-bit codes goes by how much the cache or a row of the
+    table holds a sequence: of a table that is much wider than the batch's sequences pass the columns in use.)  ``return_lse`` adds the fp32 natural-log LSE [batch, head_q].
     """
     return decoding_attn_cuda.quantized_fwd(q, k_cache, v_cache, k_scale, v_scale, cu_seq_k, is_alibi, softmax_scale, out,
                                             return_lse, block_table)

@@ -287,9 +287,9 @@ typedef struct da_prefix_decode_args {
 /* Decode attention of a batch whose sequences share their first prefix_len keys: one query token per sequence over
  * [prefix ; own keys].  The prefix is read once for the whole batch and multiplied on the tensor cores with the query
  * heads of all sequences as rows; the own keys (of any lengths, zero included) follow as in da_quant_decode_fwd, and the
- * results are joined.  Softmax weights are rounded to the type of q (fp16: or to 2^-32 of the head's largest; own keys stored as
- * codes: as in da_quant_decode_fwd), everything else is fp32.  With prefix_len = 0 and no own keys a row is zero and its LSE -inf.  The workspace needs no clearing; calls that
- * may overlap need one each.  Graph-capturable.  Refused where batch * head_q * prefix_len is past 2^44 or so.  The reference has
+ * results are joined.  Softmax weights are rounded to the type of q (8 bits for bf16, 11 for fp16, or 2^-32 of the head's
+ * largest; own keys stored as codes: as in da_quant_decode_fwd), everything else is fp32.  With prefix_len = 0 and no own
+ * keys a row is zero and its LSE -inf.  The workspace needs no clearing; calls that may overlap need one each.  Graph-capturable.  Refused where batch * head_q * prefix_len is past 2^44 or so.  The reference has
  * no counterpart. */
 int da_prefix_decode_fwd(const da_prefix_decode_args_t *args);
 size_t da_prefix_decode_workspace_bytes(const da_prefix_decode_args_t *args);
