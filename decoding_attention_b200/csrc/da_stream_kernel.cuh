@@ -22,6 +22,9 @@
 // CTA an SM that fits: 191 us for the int4 case above); and 32 heads a warp, so that a group of 32 is widened once instead
 // of twice (128 sequences of 2 048 int4 keys, 32 heads over one KV head: 51 us against 42 with two warps of 16 heads; 44 now).
 //
+// And the weights below as two fp16 parts, 22 bits, by a second multiply-add each: 128 sequences of 2 048 int4 keys, 32 heads,
+// 48 us instead of 43.
+//
 // q is brought to fp16 with a power of two per head that makes its largest element 1..2, undone in the score's factor:
 // exact, but for elements of a bf16 head below 2^-14 of its largest, which keep 2^-25 of that.  The weights w_j = p_j vs_j
 // are rounded to fp16 in units of their own, a power of two per head that is kept like the reference maximum: the largest
