@@ -27,9 +27,10 @@
 //
 // q is brought to fp16 with a power of two per head that makes its largest element 1..2, undone in the score's factor:
 // exact, but for elements of a bf16 head below 2^-14 of its largest, which keep 2^-25 of that.  The weights w_j = p_j vs_j
-// are rounded to fp16 in units of their own, a power of two per head that is kept like the reference maximum: the largest
+// are rounded to fp16 in units of their own, one factor per head that is kept like the reference maximum: the largest
 // weight so far comes to 2^7..2^15, so that a weight is off by half a step, 2^-11 of itself, or by 2^-32 of the largest.
-// (The units follow the weights and not the probabilities: a key that leads by far may have a V row of zeros.)  16-bit
+// Where it sets the units the largest is not rounded at all, which takes the error of fp16 outputs from 1.4 to 1.1 times their
+// own rounding.  (The units follow the weights and not the probabilities: a key that leads by far may have a V row of zeros.)  16-bit
 // caches: the weights are the probabilities, rounded to the cache's type, which V has and the instruction wants on both
 // sides.  Between q and o these are the only roundings to fewer bits; sums, maxima and outputs are fp32.
 //
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                         l[n][e] *= shrink;
                         if (C::kQuant) {
                             const int by = min(0, kMostScaled - exponent(v_top) - exponent(f[n][e]));
-                            f[n][e] = power2(exponent(f[n][e]) + by);
+                            f[n][e] = __uint_as_float(__float_as_uint(f[n][e]) + ((uint32_t)by << 23));  // times 2^by
                             shrink *= power2(max(-126, by));  // (past that there is nothing to keep)
                         }
 #pragma unroll
@@ -657,8 +658,8 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                         }
                 }
             if (C::kQuant && (__any_sync(0xffffffffu, wide || unset != 0))) {
-                // The weights' own reference: the largest of this tile comes to 2^7..2^8 if it has outgrown its units, or if
-                // it is the first that is not zero since the reference maximum rose (a small weight may then be the one that
+                // The weights' own reference: the largest of this tile comes to 2^7 if it has outgrown its units, or if it is
+                // the first that is not zero since the reference maximum rose (a small weight may then be the one that
                 // matters) -- as far as what has been summed up so far still fits fp32.
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -677,10 +678,11 @@ __global__ void __launch_bounds__(kStreamWarps * 32, StreamCfg<KIND, D, NT>::kTw
                         const int ex = exponent(top);
                         if (ex > -127 && ex < 128 && (ex >= 15 || ((unset >> (2 * n + e)) & 1u))) {
                             unset &= ~(1u << (2 * n + e));
-                            // (no less than -102: a V scale is at most 2^101 in these units, a probability 2^8)
+                            // To 2^7 exactly, if nothing is in the way: the weight that matters most is not rounded then.
+                            // (by: no less than -102, since a V scale is at most 2^101 in these units, a probability 2^8)
                             const int by = min(min(min(7 - ex, 126), 120 - exponent(f[n][e])), max(0, 100 - exponent(held)));
-                            const float g = power2(by);
-                            f[n][e] = power2(exponent(f[n][e]) + by);
+                            const float g = by == 7 - ex ? 128.0f / top : power2(by);
+                            f[n][e] *= g;
 #pragma unroll
                             for (int t = 0; t < MT; ++t) s[t][n][e] *= g, s[t][n][2 + e] *= g;
 #pragma unroll
